@@ -606,6 +606,31 @@ int bl_embed_pairs(const void* table, const void* pairs, int dtype, const int* i
                    const int* cu_q, const int* slots, int* prev_tokens, long long mul_prev, long long mul_cur, long long buckets,
                    float* out, int T, int d, void* stream);
 
+// Steps in which a request tries a tree of drafted tokens. Request r brings n = cu_q[r + 1] - cu_q[r] nodes (at most 64: nodes from the 65th
+// on are left alone), whose keys and values lie in its cache rows c .. c + n - 1, c = ctx_len[r] - n. mask[t]: bit i says that
+// node t sees node i of its request; a node's position is c + popcount(mask) - 1.
+// bl_attention_tree: out[t, h] = sum_j softmax_j(scale q . k_j) v_j over the committed rows (with a window those with j + window > the
+// node's position) and the nodes of mask[t] (with a window the nearest `window` of them); a row that sees nothing becomes zeros.
+// q, out [T, H * dh], caches [pages, KV, page_size, dh]; scratch: bl_attention_tree_scratch(dh) floats of this call's own, contents
+// unimportant. mask [T]. Any dtype, head size up to 256 and page size (attention_tree.cu).
+long long bl_attention_tree_scratch(int dh);
+int bl_attention_tree(const void* q, const void* k_cache, const void* v_cache, int dtype, const int* cu_q, const int* ctx_len,
+                      const long long* mask, const int* block_table, int max_pages, void* out, float* scratch, int T, int R, int H, int KV,
+                      int dh, int page_size, int window, float scale, void* stream);
+// bl_accept_tree: sampled[t] is the token that the model gives behind node t, tokens[t] what the node holds; mask[t] the bits of node t's
+// ancestors and its own. Node 0 is accepted, another node when its ancestors are and its token is the one sampled behind its
+// parent. The deepest accepted node (the lowest of several) ends the path: counts[r] nodes, path[r, 0..63] (then -1), answer[r, j] =
+// sampled[path[r, j]] (then -1). Node j of the path moves from cache row c + path[j] to c + j in all layers; k_pages and v_pages are
+// [layers][pages, KV, page_size, dh], the layers *_layer_stride elements apart.
+// bl_copy_blocks: t[layer, pairs[i][1]] = t[layer, pairs[i][0]] for tensors of `blocks` blocks of block_bytes bytes in layers that are
+// layer_bytes apart; `pairs` (and the other lists) lie in host memory and are read during the call. No target twice, none that is a source.
+int bl_accept_tree(const int* sampled, const int* tokens, const long long* mask, const int* cu_q, const int* ctx_len,
+                   const int* block_table, int max_pages, void* k_pages, void* v_pages, int elem_bytes, long long k_layer_stride,
+                   long long v_layer_stride, int layers, int KV, int page_size, int dh, int* counts, int* path, int* answer, int R,
+                   void* stream);
+int bl_copy_blocks(int n_tensors, void* const* bases, const long long* layer_bytes, const long long* block_bytes, const int* layers,
+                   const int* blocks, const int* pairs, int n_pairs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,8 +5,10 @@ sm_100a device these functions raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import itertools
 from typing import Optional
 
 import torch
@@ -2169,3 +2171,133 @@ def hyper_step(x: torch.Tensor, n: int, x_out: Optional[torch.Tensor] = None, wr
     _call(_lib().bl_hyper_step, _p(x), ll(T * d if x.dim() == 3 else 0), _p(x_out), ll(T * d), n, _p(write), _p(y), _p(y_pos), _p(y_wts),
           top, _p(read), _p(norm_w), _vec_dt(norm_w), ctypes.c_float(eps), _p(h), _dt(h) if h is not None else 0, _p(row_idx), rows, d,
           _stream())
+
+
+# ---- trees of drafted tokens, forked requests --------------------------------------------------------------------------
+
+TREE_MAX_NODES = 64       # nodes of one request in a step: what a node sees of them is a 64-bit mask
+
+
+def _here(*tensors: torch.Tensor) -> None:
+    """All on the current CUDA device, whose current stream the kernels are launched on."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError("must be CUDA tensors")
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t.device.index != now:
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{now}")
+
+
+def _fits(t: torch.Tensor, name: str, dtype, shape) -> None:
+    """The part of `_need` that needs no device."""
+    if t.dtype != dtype:
+        raise KernelError(f"{name}: must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise KernelError(f"{name}: must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name}: must be contiguous")
+
+
+def _tree_step(mask: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor):
+    """(T, R) of a step with trees."""
+    T, R = mask.shape[0], ctx_len.shape[0]
+    _fits(mask, "mask", torch.int64, (T,)); _fits(cu_q, "cu_q", torch.int32, (R + 1,)); _fits(ctx_len, "ctx_len", torch.int32, (R,))
+    if block_table.dim() != 2 or block_table.shape[0] < R:
+        raise KernelError(f"block_table: must have a row for each of the {R} requests, got {tuple(block_table.shape)}")
+    _fits(block_table, "block_table", torch.int32, block_table.shape)
+    if T > TREE_MAX_NODES * R:
+        raise KernelError(f"{T} nodes are more than {TREE_MAX_NODES} for each of {R} requests")
+    return T, R
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor,
+                   mask: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, H: int, window: int, scale: float) -> None:
+    """Attention of the nodes of a tree of drafted tokens per request over the paged cache. Request r's nodes are rows cu_q[r] ..
+    cu_q[r + 1] - 1 (at most `TREE_MAX_NODES`); their keys and values lie in its cache rows c, c + 1, .. behind its c = ctx_len[r] - nodes
+    committed ones. `mask` [T], int64: bit i of mask[t] says that node t sees node i of its request (its ancestors and itself). A node
+    sees all committed rows, with a window those j with j + window > its position c + popcount(mask) - 1, and the nodes of its mask
+    (with a window the `window` highest bits). Rows that see nothing become zeros. A cache row that is not finite spoils the
+    nodes of its own request only. Nothing is read from the host: a captured call follows what cu_q, ctx_len, mask and
+    the table hold when it is replayed."""
+    T, R = _tree_step(mask, cu_q, ctx_len, block_table)
+    if k_cache.dim() != 4:
+        raise KernelError(f"k_cache: must be [pages, kv heads, page size, head size], got {tuple(k_cache.shape)}")
+    _, KV, page_size, dh = k_cache.shape
+    if H <= 0 or H % KV != 0:
+        raise KernelError(f"{H} heads cannot share {KV} key/value heads")
+    _dt(q)
+    _fits(q, "q", q.dtype, (T, H * dh)); _fits(k_cache, "k_cache", q.dtype, k_cache.shape)
+    _fits(v_cache, "v_cache", q.dtype, k_cache.shape); _fits(out, "out", q.dtype, (T, H * dh))
+    _here(q, k_cache, v_cache, cu_q, ctx_len, mask, block_table, out)
+    lib = _lib()
+    scratch = torch.empty(_tree_scratch(dh), dtype=torch.float32, device=q.device)
+    _call(lib.bl_attention_tree, _p(q), _p(k_cache), _p(v_cache), _dt(q), _p(cu_q), _p(ctx_len), _p(mask), _p(block_table),
+          block_table.shape[1], _p(out), _p(scratch), T, R, H, KV, dh, page_size, window, ctypes.c_float(scale), _stream())
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_scratch(dh: int) -> int:
+    fn = library.load().bl_attention_tree_scratch
+    fn.restype = ctypes.c_longlong
+    return int(fn(dh))
+
+
+def accept_tree(sampled: torch.Tensor, token_ids: torch.Tensor, mask: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor,
+                k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor):
+    """Which drafted tokens the model agrees with: (counts [R], path [R, 64], tokens [R, 64]), int32. `token_ids` [T] is what the nodes
+    hold, `sampled` [T] the model's token behind each node, `mask` [T] the bits of a node's ancestors and its own (any node whose
+    mask is not its parent's with its own bit is never accepted). Node 0 of a request is accepted; another node when its
+    ancestors are and its token is the one sampled behind its parent. The deepest accepted node, the lowest of several, ends the path:
+    `counts` nodes, `path` their numbers (then -1), `tokens` what is sampled behind them (then -1). The path's keys and values move to
+    cache rows c, c + 1, .. of `k_pages` and `v_pages` [layers, pages, kv heads, page size, head size] (contiguous layers), in place; the pages
+    that hold a request's nodes must be its own. The three results are views of one buffer, counts and tokens first."""
+    T, R = _tree_step(mask, cu_q, ctx_len, block_table)
+    _fits(sampled, "sampled", torch.int32, (T,)); _fits(token_ids, "token_ids", torch.int32, (T,))
+    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape:
+        raise KernelError(f"k_pages, v_pages: must be [layers, pages, kv heads, page size, head size] alike, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    layers, pages, KV, page_size, dh = k_pages.shape
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _dt(t)
+        if t.dtype != k_pages.dtype or t.stride()[1:] != (KV * page_size * dh, page_size * dh, dh, 1) or t.stride(0) < pages * KV * page_size * dh:
+            raise KernelError(f"{name}: each layer must be contiguous, layers must not overlap, and the dtypes must agree")
+    _here(sampled, token_ids, mask, cu_q, ctx_len, k_pages, v_pages, block_table)
+    lib = _lib()
+    got = torch.empty((1 + 2 * TREE_MAX_NODES) * R, dtype=torch.int32, device=mask.device)
+    tokens, path = got[R:(1 + TREE_MAX_NODES) * R].view(R, TREE_MAX_NODES), got[(1 + TREE_MAX_NODES) * R:].view(R, TREE_MAX_NODES)
+    LL = ctypes.c_longlong
+    _call(lib.bl_accept_tree, _p(sampled), _p(token_ids), _p(mask), _p(cu_q), _p(ctx_len), _p(block_table), block_table.shape[1],
+          _p(k_pages), _p(v_pages), k_pages.element_size(), LL(k_pages.stride(0)), LL(v_pages.stride(0)), layers, KV, page_size, dh, _p(got),
+          _p(path), _p(tokens), R, _stream())
+    return got[:R], path, tokens
+
+
+def copy_blocks(tensors, pairs) -> None:
+    """t[:, target] = t[:, source] for every (source, target) of `pairs` (a list of pairs of ints) and every tensor [layers, blocks, ...] whose
+    blocks are contiguous: pages, or state slots, of all layers in one launch (a launch for every 1,024 pairs). No block may be the
+    target of two copies, or target and source. The pairs are part of the launch: a captured call copies the same ones again."""
+    flat = array.array("i", itertools.chain.from_iterable(pairs))
+    if len(flat) != 2 * len(pairs):
+        raise KernelError("pairs: must be pairs of block numbers")
+    n = len(tensors)
+    bases, layer_bytes, block_bytes = (ctypes.c_void_p * n)(), (ctypes.c_longlong * n)(), (ctypes.c_longlong * n)()
+    layers, blocks = (ctypes.c_int * n)(), (ctypes.c_int * n)()
+    for i, t in enumerate(tensors):
+        if t.dim() < 2:
+            raise KernelError(f"tensor {i}: must be [layers, blocks, ...], got {tuple(t.shape)}")
+        size = 1
+        for extent, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if extent != 1 and stride != size:
+                raise KernelError(f"tensor {i}: the blocks of a layer must be contiguous")
+            size *= extent
+        if t.shape[0] > 1 and t.stride(0) < size:
+            raise KernelError(f"tensor {i}: layers must not overlap")
+        item = t.element_size()
+        bases[i], layer_bytes[i] = t.data_ptr(), t.stride(0) * item
+        layers[i], blocks[i] = t.shape[0], t.shape[1]
+        block_bytes[i] = size // max(1, t.shape[1]) * item
+    if n == 0 or len(flat) == 0:
+        return
+    _here(*tensors)
+    at, _ = flat.buffer_info()
+    _call(_lib().bl_copy_blocks, n, bases, layer_bytes, block_bytes, layers, blocks, ctypes.c_void_p(at), len(pairs), _stream())
