@@ -617,6 +617,14 @@ long long bl_attention_tree_scratch(int dh);
 int bl_attention_tree(const void* q, const void* k_cache, const void* v_cache, int dtype, const int* cu_q, const int* ctx_len,
                       const long long* mask, const int* block_table, int max_pages, void* out, float* scratch, int T, int R, int H, int KV,
                       int dh, int page_size, int window, float scale, void* stream);
+// bl_attention_tree_tc: the same for bfloat16, head sizes 64 and 128 and pages of 16 on tcgen05 (attention_tree_tc.cu); q, the caches, out and
+// scratch (bl_attention_tree_tc_scratch(dh) floats) 16-byte aligned, n_pages the caches' first dimension.
+int bl_attention_tree_tc_supported(int H, int KV, int dh, int page_size);
+long long bl_attention_tree_tc_scratch(int dh);
+int bl_attention_tree_tc(const void* q, const void* k_cache, const void* v_cache, const int* cu_q, const int* ctx_len,
+                         const long long* mask, const int* block_table, int max_pages, void* out, float* scratch, int T, int R, int n_pages,
+                         int H, int KV, int dh, int page_size, int window, float scale, void* stream);
+int bl_attention_tree_tc_status(int* status);
 // bl_accept_tree: sampled[t] is the token that the model gives behind node t, tokens[t] what the node holds; mask[t] the bits of node t's
 // ancestors and its own. Node 0 is accepted, another node when its ancestors are and its token is the one sampled behind its
 // parent. The deepest accepted node (the lowest of several) ends the path: counts[r] nodes, path[r, 0..63] (then -1), answer[r, j] =

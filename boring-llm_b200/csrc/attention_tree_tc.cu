@@ -1,0 +1,572 @@
+// Attention of the nodes of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores: bfloat16, head sizes 64
+// and 128, pages of 16. Formula, masks and positions are those of attention_tree.cu, the line of work that the blocks share out and the merge
+// of units that are cut those of attention_tree.cuh (128 rows, 128 keys).
+//
+// One block per SM walks its part of the line, segment by segment (a segment: some key blocks of one unit), through one pipeline that
+// does not drain between segments:
+//   copies    q rows of a unit as one box per 64 dimensions (pairs of node and query head are rows of q as they lie); of a key block one
+//             box per page and tensor: 16 keys as two groups of 8 rows x (dh / 64) atoms of 128 bytes, so that a key block lies in shared
+//             memory as [16 groups][atoms][8 rows][128 bytes], which the operand descriptors walk with a group stride of atoms x 1,024. Two
+//             warps issue the boxes of the keys and two those of the values (a box costs its thread about 0.1 us). A page that no node may
+//             see is asked for behind the end of the cache: zeros arrive.
+//   S = Q K^T tcgen05.mma, M 128 x N 128 x K dh, into one of three buffers of tensor memory;
+//   softmax   four warps, a thread per row: maximum, then P = 2^(s - m) as bfloat16 over the upper half of its scores; m moves only when
+//             a block's maximum passes it by 2^8 (then O is rescaled in tensor memory). Warps without rows pass their turn;
+//   O += P V  tcgen05.mma, A from tensor memory, V as it lies.
+// The scores of up to two further blocks are computed meanwhile. Only blocks with nodes, or at the edge of a window, look at masks.
+// Values behind the request's last row, in a page that was copied, are set to zero (0 x whatever an old request left must stay 0).
+// P is rounded to bfloat16 (half a step, 2^-8 of each weight, as the operand of a bfloat16 product must be); the sum is of the 32-bit values.
+//
+// Every wait on an mbarrier is bounded; a block whose bound runs out records a code in a status word
+// (bl_attention_tree_tc_status), its warps leave their loops, its copies are waited for, its tensor memory is freed.
+#include "tcgen05.cuh"
+#include "attention_tree.cuh"
+#include <atomic>
+
+namespace {
+
+constexpr const char* WHO = "bl_attention_tree_tc";
+constexpr int ROWS = 128, KEYS = 128, PAGE = 16, PAGES = KEYS / PAGE;
+constexpr int SBUFS = 3, TMEM_COLS = 512, COL_P = KEYS / 2, COL_O = SBUFS * KEYS;
+constexpr int ROW_WARPS = 4, COPY_WARPS = 4;                             // then: S, PV, copies, q
+constexpr int WARP_S = ROW_WARPS, WARP_PV = WARP_S + 1, WARP_COPY = WARP_PV + 1, WARP_Q = WARP_COPY + COPY_WARPS;
+constexpr int THREADS = 32 * (WARP_Q + 1);
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+
+template <int DH_>
+struct Shape {
+    static constexpr int DH = DH_, ATOMS = DH / 64, STAGES = DH == 64 ? 6 : 3;
+    static constexpr int GROUP = ATOMS * 1024;                           // eight keys
+    static constexpr int Q_BYTES = ATOMS * ROWS * 128, KV_BYTES = KEYS / 8 * GROUP;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_BARS = OFF_V + STAGES * KV_BYTES;
+    static constexpr int SMEM_BYTES = OFF_BARS + 512;
+    static_assert(SMEM_BYTES <= 227 * 1024 && COL_O + DH <= TMEM_COLS, "shape does not fit an SM");
+};
+
+__device__ int g_status = 0;           // 0 = fine; else the code of the first wait that ran out
+
+struct Params {
+    TreeLine line;
+    __nv_bfloat16* out; const unsigned long long* mask; const int* table; int max_pages;
+    int H, G, no_group; float scale_log2; float* scratch;                // no_group: the first group of 8 rows behind the cache
+};
+
+__device__ __forceinline__ bool wait_nap(uint32_t bar, uint32_t parity, volatile int* give_up, int code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*give_up) return false;
+        __nanosleep(20);
+    }
+    *give_up = 1;
+    atomicCAS(&g_status, 0, code);
+    return false;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(0), "r"(c3) : "memory");
+}
+// D (+)= A . B with the A operand in tensor memory (lane = row, a 32-bit column = two bfloat16 along K)
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// tcgen05.wait::ld tied to the registers of the load it completes: nothing that reads them may be moved above it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {                          // 2^x on the special-function unit (about 2 ulp; 2^-inf = 0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<unsigned*>(&v);
+}
+// An operand in shared memory, 128-byte swizzle, its groups of 8 rows `group` bytes apart (tcgen05.cuh's form has 1,024).
+__device__ __forceinline__ uint64_t desc_groups(uint32_t addr, int group) {
+    return (smem_desc(addr) & ~((uint64_t)0x3FFF << 32)) | ((uint64_t)(group >> 4) << 32);
+}
+
+// kind::f16 instruction descriptors: D 32-bit, A and B bfloat16, N >> 3 at bit 17, M >> 4 at bit 24; bit 16: B lies keys x head size.
+constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+
+// A counter of blocks as (index mod N, parity of the index div N).
+template <int N> struct Ring {
+    int at = 0; uint32_t par = 0;
+    __device__ __forceinline__ void next() { if (++at == N) { at = 0; par ^= 1; } }
+};
+
+template <class S>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const Params p) {
+    constexpr int DH = S::DH, ATOMS = S::ATOMS, STAGES = S::STAGES, GROUP = S::GROUP, KV_BYTES = S::KV_BYTES;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    if (threadIdx.x == 0) { tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v); }
+    const uint32_t base = smem_u32(smem), bars = base + S::OFF_BARS;
+    const uint32_t full_q = bars, q_free = bars + 8;
+    const uint32_t s_done0 = bars + 16, p_ready0 = s_done0 + 8 * SBUFS, buf_free0 = p_ready0 + 8 * SBUFS;
+    const uint32_t full_k0 = buf_free0 + 8 * SBUFS, k_free0 = full_k0 + 8 * STAGES, full_v0 = k_free0 + 8 * STAGES, v_free0 = full_v0 + 8 * STAGES;
+    volatile int* give_up = reinterpret_cast<volatile int*>(smem + S::OFF_BARS + 320);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::OFF_BARS + 328);
+    long long* s_total = reinterpret_cast<long long*>(smem + S::OFF_BARS + 336);
+    TreePlace* s_place = reinterpret_cast<TreePlace*>(smem + S::OFF_BARS + 352);
+    static_assert(16 + 8 * (3 * SBUFS + 4 * STAGES) <= 320 && 352 + sizeof(TreePlace) <= 512, "barriers overlap");
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        *give_up = (base & 1023u) ? 1 : 0;                               // the swizzled tiles need 1024-byte alignment
+        if (base & 1023u) atomicCAS(&g_status, 0, 9);
+        mbar_init(full_q, 1); mbar_init(q_free, 1);
+        for (int i = 0; i < SBUFS; ++i) { mbar_init(s_done0 + 8 * i, 1); mbar_init(p_ready0 + 8 * i, ROWS); mbar_init(buf_free0 + 8 * i, 1); }
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(full_k0 + 8 * i, COPY_WARPS / 2); mbar_init(k_free0 + 8 * i, 1);
+            mbar_init(full_v0 + 8 * i, COPY_WARPS / 2); mbar_init(v_free0 + 8 * i, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Tensor memory before the wait for the kernel before (which has taken its own before it let this one start).
+    if (warp == WARP_S) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32((const void*)tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    bl_pdl_wait();
+    bl_pdl_trigger();
+    if (warp == 0) {
+        const long long total = tree_total<KEYS>(p.line);
+        const int parts = tree_parts(total, gridDim.x);
+        if (total > 0 && (int)blockIdx.x < parts) {
+            const TreePlace w = tree_find<KEYS>(p.line, tree_part(total, parts, blockIdx.x));
+            if (lane == 0) *s_place = w;
+        }
+        if (lane == 0) *s_total = total;
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const long long total = *s_total;
+    const int parts = tree_parts(total, gridDim.x);
+    const bool busy = total > 0 && (int)blockIdx.x < parts;
+    TreePlace w = *s_place;
+    long long left = busy ? tree_part(total, parts, blockIdx.x + 1) - tree_part(total, parts, blockIdx.x) : 0;
+    bool ok = !*give_up;
+    // the segments of this block's part, one after the other: f(segment, its key blocks)
+    auto segments = [&](auto f) {
+        for (int seg = 0; ok && left > 0; ++seg) {
+            const int n = (int)min(left, (long long)(w.q.b0 + w.q.nb - w.b));
+            f(seg, n);
+            left -= n;
+            if (left > 0) tree_next_unit<KEYS>(p.line, w);
+        }
+    };
+
+    if (warp >= WARP_COPY && warp < WARP_COPY + COPY_WARPS) {
+        // ================= copies of half a key block's pages: lanes 0..3 look up a page each, one thread issues
+        const bool keys = ((warp - WARP_COPY) & 1) == 0;
+        const int half = (warp - WARP_COPY) >> 1;
+        const CUtensorMap* map = keys ? &map_k : &map_v;
+        const uint32_t full0 = keys ? full_k0 : full_v0, free0 = keys ? k_free0 : v_free0;
+        const uint32_t dst0 = base + (keys ? S::OFF_K : S::OFF_V) + half * (KV_BYTES / 2);
+        auto group_of = [&]() -> int {                                   // lane's page of the block w.b, as a group of 8 rows of the cache
+            const int first = w.b * KEYS + (half * (PAGES / 2) + (lane & 3)) * PAGE;
+            if (first > w.q.c + w.q.n - 1 || first + PAGE - 1 < w.q.lo) return p.no_group;
+            return (p.table[(size_t)w.r * p.max_pages + first / PAGE] * p.line.KV + w.kvh) * 2;
+        };
+        Ring<STAGES> ring;
+        int used = 0;
+        ok = __all_sync(0xffffffffu, ok);
+        int group = left > 0 ? group_of() : 0;
+        for (long long i = 0; ok && left > 0; ++i) {
+            int group_next = 0;                                          // on its way during this block's copies
+            const uint32_t bar = full0 + 8 * ring.at, dst = dst0 + ring.at * KV_BYTES;
+            if (--left > 0) {
+                if (++w.b == w.q.b0 + w.q.nb) tree_next_unit<KEYS>(p.line, w);
+                group_next = group_of();
+            }
+            if (i >= STAGES) {
+                if (lane == 0) ok = wait_nap(free0 + 8 * ring.at, ring.par ^ 1, give_up, keys ? 3 : 7);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            int g[PAGES / 2];
+#pragma unroll
+            for (int pg = 0; pg < PAGES / 2; ++pg) g[pg] = __shfl_sync(0xffffffffu, group, pg);
+            if (elect_one()) {
+                mbar_expect_tx(bar, KV_BYTES / 2);
+#pragma unroll
+                for (int pg = 0; pg < PAGES / 2; ++pg) tma_load_4d(dst + pg * 2 * GROUP, map, bar, g[pg]);
+            }
+            __syncwarp();
+            used = used < STAGES ? used + 1 : STAGES;
+            ring.next();
+            group = group_next;
+        }
+        // a block that gave up lets its own copies land before its shared memory goes to the next block
+        if (lane == 0 && *give_up && !(base & 1023u)) {
+            for (int k = 0; k < used; ++k) {                             // the last `used` copies
+                if (ring.at == 0) { ring.at = STAGES; ring.par ^= 1; }
+                --ring.at;
+                mbar_wait_landed(full0 + 8 * ring.at, ring.par, 1u << 16);
+            }
+        }
+    } else if (warp == WARP_Q) {
+        int loaded = 0;
+        segments([&](int seg, int) {
+            if (seg > 0) {
+                if (lane == 0) ok = wait_nap(q_free, (uint32_t)(seg - 1) & 1, give_up, 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+            }
+            if (elect_one()) {
+                mbar_expect_tx(full_q, (uint32_t)(ATOMS * p.G * p.line.npt * 128));
+#pragma unroll
+                for (int a = 0; a < ATOMS; ++a)
+                    tma_load_3d(base + a * ROWS * 128, &map_q, full_q, a * 64, w.kvh * p.G, w.q.begin + w.tile * p.line.npt);
+            }
+            __syncwarp();
+            ++loaded;
+        });
+        if (lane == 0 && *give_up && loaded > 0) mbar_wait_landed(full_q, (uint32_t)(loaded - 1) & 1, 1u << 16);
+    } else if (warp == WARP_S) {
+        if (ok && elect_one()) {
+            Ring<STAGES> st;
+            Ring<SBUFS> buf;
+            long long i = 0;
+            segments([&](int seg, int n) {
+                ok = wait_nap(full_q, (uint32_t)seg & 1, give_up, 2);
+                for (int j = 0; ok && j < n; ++j, ++i) {
+                    ok = wait_nap(full_k0 + 8 * st.at, st.par, give_up, 6);
+                    if (ok && i >= SBUFS) ok = wait_nap(buf_free0 + 8 * buf.at, buf.par ^ 1, give_up, 4);
+                    if (!ok) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int at = 0; at < ATOMS; ++at) {
+                        const uint64_t a = smem_desc(base + at * ROWS * 128);
+                        const uint64_t b = desc_groups(base + S::OFF_K + st.at * KV_BYTES + at * 1024, GROUP);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma_bf16(tmem + buf.at * KEYS, a + 2 * k, b + 2 * k, IDESC_S, (at | k) != 0);
+                    }
+                    umma_commit(k_free0 + 8 * st.at);
+                    umma_commit(s_done0 + 8 * buf.at);
+                    if (j + 1 == n) umma_commit(q_free);
+                    st.next(); buf.next();
+                }
+            });
+        }
+        __syncwarp();
+    } else if (warp == WARP_PV) {
+        if (ok && elect_one()) {
+            Ring<STAGES> st;
+            Ring<SBUFS> buf;
+            segments([&](int, int n) {
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = wait_nap(full_v0 + 8 * st.at, st.par, give_up, 5) &&
+                         mbar_wait_bounded(p_ready0 + 8 * buf.at, buf.par, WAIT_LIMIT, give_up, &g_status, 12);
+                    if (!ok) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int at = 0; at < ATOMS; ++at) {                 // 64 dimensions of the head at a time
+                        const uint64_t bv = desc_groups(base + S::OFF_V + st.at * KV_BYTES + at * 1024, GROUP);
+#pragma unroll
+                        for (int kk = 0; kk < KEYS / 16; ++kk)           // 16 keys a step: 8 columns of P, two groups of V
+                            umma_bf16_ts(tmem + COL_O + at * 64, tmem + buf.at * KEYS + COL_P + kk * 8, bv + (uint64_t)(kk * (2 * GROUP >> 4)), IDESC_PV,
+                                         (kk == 0 && j == 0) ? 0u : 1u);
+                    }
+                    umma_commit(buf_free0 + 8 * buf.at);
+                    umma_commit(v_free0 + 8 * st.at);
+                    st.next(); buf.next();
+                }
+            });
+        }
+        __syncwarp();
+    } else {
+        // ================= the row warps: thread = row of the tile = lane of tensor memory
+        constexpr float RESCALE = 8.f;
+        const int row = warp * 32 + lane, node = row / p.G;
+        const uint32_t lane_off = (uint32_t)(warp * 32) << 16, t_o = tmem + COL_O + lane_off;
+        Ring<STAGES> st;
+        Ring<SBUFS> buf;
+        // Waits for the product P V of the block before `buf`'s. A wait for a phase is valid while the barrier is at most one phase
+        // behind it (phases are told apart by parity alone): the barrier is the score buffer's, whose phase before was that
+        // of four blocks ago (three after P has been posted), and the scores of a block that has been looked at were issued only
+        // after the product of three blocks before it had been added. It cannot be ahead: the product three blocks on waits for this warp.
+        auto product_done = [&](Ring<SBUFS> of, int code) -> bool {
+            if (of.at == 0) { of.at = SBUFS; of.par ^= 1; }
+            --of.at;
+            bool fine = mbar_wait_bounded(buf_free0 + 8 * of.at, of.par, WAIT_LIMIT, give_up, &g_status, code);
+            fine = __all_sync(0xffffffffu, fine);
+            if (fine) fence_after_sync();
+            return fine;
+        };
+        segments([&](int seg, int n) {
+            const TreeRequest q = w.q;
+            const int node0 = w.tile * p.line.npt, nodes = min(p.line.npt, q.n - node0), hi = q.c + q.n - 1;
+            const bool valid = node < nodes, warp_rows = warp * 32 < nodes * p.G;
+            const size_t tok = (size_t)q.begin + node0 + node;
+            unsigned long long seen = 0;
+            int lo = q.c;                                                // a row that the tile does not have sees nothing that matters
+            if (valid) {
+                const unsigned long long m = p.mask[tok];
+                const int pos = q.c + max(__popcll(q.n < 64 ? m & ((1ULL << q.n) - 1) : m) - 1, 0);
+                seen = tree_mask(m, q.n, p.line.window);
+                lo = p.line.window > 0 ? min(max(0, pos - p.line.window + 1), q.c) : 0;
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; ++j) {
+                const int k0 = (w.b + j) * KEYS;
+                const uint32_t t_s = tmem + buf.at * KEYS + lane_off, t_p = t_s + COL_P;
+                ok = mbar_wait_bounded(s_done0 + 8 * buf.at, buf.par, WAIT_LIMIT, give_up, &g_status, 8) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                fence_after_sync();
+                if (warp_rows) {
+                    const bool all_seen = k0 + KEYS <= q.c && k0 >= lo;
+                    auto mask = [&](uint32_t (&s)[32], int c) {          // a key that the row does not see becomes -inf
+                        const unsigned bits = tree_bits(seen, q.c, lo, k0 + 32 * c);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) s[x] = (bits >> x) & 1u ? s[x] : 0xff800000u;
+                    };
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto chunk_max = [&](uint32_t (&s)[32], int c) {
+                        if (!all_seen) mask(s, c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) mx[(x >> 1) & 3] = max3(mx[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+                    };
+                    // first pass: the maximum; the next 32 scores on their way meanwhile
+                    uint32_t sa[32], sb[32];
+                    tmem_ld32(t_s, sa);
+#pragma unroll 1
+                    for (int cp = 0; cp < 2; ++cp) {
+                        tmem_ld_wait(sa); tmem_ld32(t_s + (2 * cp + 1) * 32, sb); chunk_max(sa, 2 * cp);
+                        tmem_ld_wait(sb); tmem_ld32(t_s + 64, sa); chunk_max(sb, 2 * cp + 1);
+                    }
+                    const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+                    if (__any_sync(0xffffffffu, m_new > m + RESCALE)) {
+                        const float alpha = ex2(m - (m_new == -INFINITY ? 0.f : m_new));
+                        m = m_new;
+                        l *= alpha;
+                        if (j > 0) {                                     // what has been added so far moves to the new reference
+                            ok = product_done(buf, 11);
+                            if (!ok) return;
+#pragma unroll 1
+                            for (int h = 0; h < DH / 32; ++h) {
+                                uint32_t v[32];
+                                tmem_ld32(t_o + h * 32, v);
+                                tmem_ld_wait(v);
+                                uint32_t a16[16], b16[16];
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) {
+                                    a16[x] = __float_as_uint(__uint_as_float(v[x]) * alpha);
+                                    b16[x] = __float_as_uint(__uint_as_float(v[16 + x]) * alpha);
+                                }
+                                tmem_st16(t_o + h * 32, a16);
+                                tmem_st16(t_o + h * 32 + 16, b16);
+                            }
+                        }
+                    }
+                    const float m_use = m == -INFINITY ? 0.f : m;
+                    uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+                    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), minus_m2 = f2_pack(-m_use, -m_use);
+                    // second pass, chunks 3 (still in sb), 2, 1, 0: P of chunk c goes over scores that are in registers by then
+                    auto chunk_exp = [&](uint32_t (&s)[32], int c) {
+                        if (!all_seen) mask(s, c);
+                        float x[32];
+#pragma unroll
+                        for (int y = 0; y < 32; y += 2)
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), scale2, minus_m2), x[y], x[y + 1]);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[y]));
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            sum2[y & 1] = f2_add(sum2[y & 1], f2_pack(x[2 * y], x[2 * y + 1]));
+                            pk[y] = pack_bf16(x[2 * y], x[2 * y + 1]);
+                        }
+                        tmem_st16(t_p + 16 * c, pk);
+                    };
+#pragma unroll 1
+                    for (int cp = 1; cp >= 0; --cp) {
+                        chunk_exp(sb, 2 * cp + 1);
+                        tmem_ld_wait(sa);
+                        if (cp) tmem_ld32(t_s + 32, sb);
+                        chunk_exp(sa, 2 * cp);
+                        if (cp) { tmem_ld_wait(sb); tmem_ld32(t_s, sa); }
+                    }
+                    float s_a, s_b, s_c, s_d;
+                    f2_unpack(sum2[0], s_a, s_c);
+                    f2_unpack(sum2[1], s_b, s_d);
+                    l += (s_a + s_b) + (s_c + s_d);
+                }
+                // the last page of the request: values behind its last row become zeros
+                if (hi >= k0 && hi < k0 + KEYS && (hi + 1) % PAGE != 0) {
+                    ok = mbar_wait_bounded(full_v0 + 8 * st.at, st.par, WAIT_LIMIT, give_up, &g_status, 10) && ok;
+                    if (ok) {
+                        const int r0 = hi + 1 - k0, rows = PAGE - r0 % PAGE;             // rows r0 .. r0 + rows - 1 of the stage
+                        for (int x = row; x < rows * ATOMS * 8; x += ROWS) {
+                            const int key = r0 + x / (ATOMS * 8), piece = x % (ATOMS * 8);
+                            *reinterpret_cast<uint4*>(smem + S::OFF_V + st.at * KV_BYTES + (key >> 3) * GROUP + (piece >> 3) * 1024 + (key & 7) * 128 + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tmem_st_wait();
+                fence_before_sync();
+                mbar_arrive(p_ready0 + 8 * buf.at);
+                st.next(); buf.next();
+            }
+            // the unit's outputs (against m, not divided by l yet), once its last product has been added
+            ok = __all_sync(0xffffffffu, ok) && product_done(buf, 13);
+            if (!ok) return;
+            const bool whole = n == q.nb;
+            const float inv = whole ? (l > 0.f ? 1.0f / l : 0.f) : 1.0f;
+            const size_t slot = 2 * (size_t)blockIdx.x + (seg == 0 ? 0 : 1);
+            float* part = p.scratch + (slot * ROWS + row) * DH;
+            __nv_bfloat16* dst = p.out + (tok * p.H + w.kvh * p.G + row - node * p.G) * DH;
+            if (warp_rows) {
+#pragma unroll 1
+                for (int h = 0; h < DH / 32; ++h) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + h * 32, v);
+                    tmem_ld_wait(v);
+                    if (valid && whole) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8) {
+                            float f[8];
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) f[y] = __uint_as_float(v[x + y]) * inv;
+                            *reinterpret_cast<uint4*>(dst + h * 32 + x) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+                        }
+                    } else if (valid) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(part + h * 32 + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (valid && !whole)
+                *reinterpret_cast<float2*>(p.scratch + (size_t)2 * gridDim.x * ROWS * DH + (slot * ROWS + row) * 2) = make_float2(m, l);
+            fence_before_sync();                                         // the outputs have been read: the next unit's first product may write them
+        });
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == WARP_S) {
+        __syncwarp();
+        fence_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+int make_map(CUtensorMap* map, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    BlEncodeTiled enc = bl_tensor_map_encoder();
+    if (enc == nullptr) BL_FAIL("%s: cuTensorMapEncodeTiled is not available from the driver", WHO);
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box, ones,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) BL_FAIL("%s: cuTensorMapEncodeTiled failed with code %d", WHO, (int)r);
+    return 0;
+}
+
+template <class S>
+int launch(const void* q, const void* k_cache, const void* v_cache, const Params& p, int T, int blocks, cudaStream_t stream) {
+    constexpr cuuint64_t DH = S::DH;
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t q_dims[3] = {DH, (cuuint64_t)p.H, (cuuint64_t)T}, q_strides[2] = {DH * 2, (cuuint64_t)p.H * DH * 2};
+    const cuuint32_t q_box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.line.npt};
+    const cuuint64_t dims[4] = {64, 8, (cuuint64_t)S::ATOMS, (cuuint64_t)p.no_group}, strides[3] = {DH * 2, 128, 8 * DH * 2};
+    const cuuint32_t box[4] = {64, 8, (cuuint32_t)S::ATOMS, 2};
+    if (make_map(&mq, q, 3, q_dims, q_strides, q_box) || make_map(&mk, k_cache, 4, dims, strides, box) || make_map(&mv, v_cache, 4, dims, strides, box)) return 1;
+    static std::atomic<bool> configured{false};
+    if (!configured) {
+        BL_CUDA(cudaFuncSetAttribute(attention_tree_tc_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES));
+        configured = true;
+    }
+    BL_CUDA(bl_launch_dependent(attention_tree_tc_kernel<S>, dim3(blocks), dim3(THREADS), (size_t)S::SMEM_BYTES, stream, mq, mk, mv, p));
+    BL_CHECK_LAUNCH("bl_attention_tree_tc");
+    if (blocks > 1) {
+        TreeMerge<__nv_bfloat16> mg{p.line, p.scratch, p.out, blocks, S::DH, p.H, p.G};
+        BL_CUDA(bl_launch_dependent(tree_merge_kernel<ROWS, KEYS, __nv_bfloat16>, dim3(blocks - 1, ROWS / 8), dim3(256), 0, stream, mg));
+        BL_CHECK_LAUNCH("bl_attention_tree_tc (merge)");
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int bl_attention_tree_tc_supported(int H, int KV, int dh, int page_size) {
+    return (dh == 64 || dh == 128) && page_size == PAGE && KV > 0 && H > 0 && H % KV == 0 && H / KV <= ROWS;
+}
+extern "C" long long bl_attention_tree_tc_scratch(int dh) { return (long long)tree_scratch_floats(bl_device_sms(), ROWS, dh); }
+
+extern "C" int bl_attention_tree_tc(const void* q, const void* k_cache, const void* v_cache, const int* cu_q, const int* ctx_len,
+                                    const long long* mask, const int* block_table, int max_pages, void* out, float* scratch, int T, int R,
+                                    int n_pages, int H, int KV, int dh, int page_size, int window, float scale, void* stream) {
+    if (T == 0 || R == 0) return 0;
+    if (!bl_attention_tree_tc_supported(H, KV, dh, page_size))
+        BL_FAIL("%s: %d heads of %d on %d key/value heads with pages of %d are not built (64 or 128, pages of 16)", WHO, H, dh, KV, page_size);
+    if (T < 0 || R < 0 || max_pages <= 0 || n_pages <= 0 || window < 0 || (long long)n_pages * KV * 2 > 0x7ffffff0LL)
+        BL_FAIL("%s: bad sizes T=%d R=%d pages=%d table=%d window=%d", WHO, T, R, n_pages, max_pages, window);
+    if (!(scale > 0.f)) BL_FAIL("%s: the scale of the scores must be positive (got %g)", WHO, (double)scale);
+    if (scratch == nullptr) BL_FAIL("%s: no scratch", WHO);
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch) & 15)
+        BL_FAIL("%s: q, the caches, out and scratch must be 16-byte aligned", WHO);
+    const int G = H / KV, npt = ROWS / G < TREE_MAX_NODES ? ROWS / G : TREE_MAX_NODES;
+    Params p{TreeLine{cu_q, ctx_len, R, KV, window, npt}, (__nv_bfloat16*)out, reinterpret_cast<const unsigned long long*>(mask), block_table, max_pages,
+             H, G, n_pages * KV * 2, scale * 1.4426950408889634f, scratch};
+    if (dh == 64) return launch<Shape<64>>(q, k_cache, v_cache, p, T, bl_device_sms(), (cudaStream_t)stream);
+    return launch<Shape<128>>(q, k_cache, v_cache, p, T, bl_device_sms(), (cudaStream_t)stream);
+}
+
+// Reads and clears the status word: 0 when no block has given up on a wait since the last call. Codes: 1 q to be read, 2 q, 3 / 7 a stage of keys /
+// values to become free, 4 a buffer of scores to become free, 5 values, 6 keys, 8 scores, 10 values (row warps), 11 / 13 the output, 12 P, 9 shared
+// memory not 1024-byte aligned. Synchronises the device.
+extern "C" int bl_attention_tree_tc_status(int* status) {
+    int v = 0, zero = 0;
+    BL_CUDA(cudaMemcpyFromSymbol(&v, g_status, sizeof(int)));
+    if (v != 0) BL_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
+    *status = v;
+    return 0;
+}

@@ -913,7 +913,8 @@ def check_status() -> None:
                      ("bl_gemm_tc_cols", _lib().bl_gemm_tc_cols_status),
                      ("bl_gemm_tc_splitk", _lib().bl_gemm_tc_splitk_status), ("bl_gemm_tc_few", _lib().bl_gemm_tc_few_status),
                      ("bl_gemm_tc_experts", _lib().bl_gemm_tc_experts_status),
-                     ("bl_attention_decode_tma", _lib().bl_attention_decode_tma_status)):
+                     ("bl_attention_decode_tma", _lib().bl_attention_decode_tma_status),
+                     ("bl_attention_tree_tc", _lib().bl_attention_tree_tc_status)):
         v = ctypes.c_int(0)
         _call(fn, ctypes.byref(v))
         if v.value != 0:
@@ -2231,14 +2232,32 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _fits(v_cache, "v_cache", q.dtype, k_cache.shape); _fits(out, "out", q.dtype, (T, H * dh))
     _here(q, k_cache, v_cache, cu_q, ctx_len, mask, block_table, out)
     lib = _lib()
-    scratch = torch.empty(_tree_scratch(dh), dtype=torch.float32, device=q.device)
+    if attention_tree_tc_supported(q, k_cache, v_cache, out, H):
+        scratch = torch.empty(_tree_scratch(dh, True), dtype=torch.float32, device=q.device)
+        _call(lib.bl_attention_tree_tc, _p(q), _p(k_cache), _p(v_cache), _p(cu_q), _p(ctx_len), _p(mask), _p(block_table), block_table.shape[1],
+              _p(out), _p(scratch), T, R, k_cache.shape[0], H, KV, dh, page_size, window, ctypes.c_float(scale), _stream())
+        return
+    scratch = torch.empty(_tree_scratch(dh, False), dtype=torch.float32, device=q.device)
     _call(lib.bl_attention_tree, _p(q), _p(k_cache), _p(v_cache), _dt(q), _p(cu_q), _p(ctx_len), _p(mask), _p(block_table),
           block_table.shape[1], _p(out), _p(scratch), T, R, H, KV, dh, page_size, window, ctypes.c_float(scale), _stream())
 
 
+def attention_tree_tc_supported(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, H: int) -> bool:
+    """Whether `attention_tree` runs these operands on the tensor cores: bfloat16, 16-byte aligned, head size 64 or 128, pages of 16."""
+    _, KV, page_size, dh = k_cache.shape
+    return (q.dtype == torch.bfloat16 and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
+            and _tree_tc_built(H, KV, dh, page_size))
+
+
 @functools.lru_cache(maxsize=None)
-def _tree_scratch(dh: int) -> int:
-    fn = library.load().bl_attention_tree_scratch
+def _tree_tc_built(H: int, KV: int, dh: int, page_size: int) -> bool:
+    return bool(library.load().bl_attention_tree_tc_supported(H, KV, dh, page_size))
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_scratch(dh: int, tc: bool) -> int:
+    lib = library.load()
+    fn = lib.bl_attention_tree_tc_scratch if tc else lib.bl_attention_tree_scratch
     fn.restype = ctypes.c_longlong
     return int(fn(dh))
 

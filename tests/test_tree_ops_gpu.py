@@ -336,3 +336,10 @@ def test_draft_step_from_scores_to_pages():
         before = after.run()
         after.table = fork
         assert torch.equal(after.run(), before)
+
+
+@pytest.fixture(autouse=True)
+def waits_ended():
+    """No block has given up on a bounded wait."""
+    yield
+    ops().check_status()
