@@ -60,8 +60,8 @@ template <typename TT, bool VEC, int NV>
 __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kernel(const Params<TT> p) {
     extern __shared__ __align__(16) float sm[];
     __shared__ long long offs[2][KEYS];                                  // where the keys of this block and the next lie
-    __shared__ TreePlace s_place;
-    __shared__ long long s_total;
+    __shared__ TreeShare s_share;
+    __shared__ int s_ends[32];
     const int dp = (p.dh + 3) & ~3, ld = dp + 4;
     float* qs = sm;                                                      // [ROWS][ld]
     float* ks = qs + ROWS * ld;                                          // [KEYS][ld]
@@ -71,25 +71,20 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
     bl_pdl_wait();
     bl_pdl_trigger();
     if (tid < 32) {
-        const long long total = tree_total<KEYS>(p.line);
-        const int parts = tree_parts(total, gridDim.x);
-        if (total > 0 && (int)blockIdx.x < parts) {
-            const TreePlace w = tree_find<KEYS>(p.line, tree_part(total, parts, blockIdx.x));
-            if (tid == 0) s_place = w;
+        const TreeShare s = tree_share<KEYS, 1, 0>(p.line, gridDim.x, blockIdx.x, s_ends);
+        if (tid == 0) {
+            s_share = s;
+            reinterpret_cast<TreeCut*>(p.scratch)[blockIdx.x] = s.cut;
         }
-        if (tid == 0) s_total = total;
     }
     __syncthreads();
-    const long long total = s_total;
-    const int parts = tree_parts(total, gridDim.x);
-    if (total == 0 || (int)blockIdx.x >= parts) return;
-    TreePlace w = s_place;
-    long long left = tree_part(total, parts, blockIdx.x + 1) - tree_part(total, parts, blockIdx.x);
+    TreePlace w = s_share.place;
+    int left = s_share.left;
     const long long page_stride = (long long)p.line.KV * p.page_size * p.dh;
 
     for (bool first = true; left > 0; first = false) {
         const TreeRequest& rq = w.q;
-        const int n_blocks = (int)min(left, (long long)(rq.b0 + rq.nb - w.b));
+        const int n_blocks = min(left, rq.b0 + rq.nb - w.b);
         const int node0 = w.tile * p.line.npt, nodes = min(p.line.npt, rq.n - node0);
         const int* table = p.table + (size_t)w.r * p.max_pages;
         const int hi = rq.c + rq.n - 1;
@@ -209,23 +204,30 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
         cp_wait<0>();
         const bool whole = n_blocks == rq.nb;
         const size_t slot = 2 * (size_t)blockIdx.x + (first ? 0 : 1);
-        float* part = p.scratch + slot * ROWS * p.dh;
-        float* stats = p.scratch + (size_t)2 * gridDim.x * ROWS * p.dh + slot * ROWS * 2;
+        float* part = tree_outputs(p.scratch, gridDim.x) + slot * ROWS * p.dh;
+        float* stats = tree_stats(p.scratch, gridDim.x, ROWS, p.dh) + slot * ROWS * 2;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const int row = ty * 4 + a, node = row / p.G;
             if (node >= nodes) continue;
-            const float inv = whole ? (l[a] > 0.f ? 1.0f / l[a] : 0.f) : 1.0f;
-            TT* dst = p.out + ((size_t)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh;
+            if (whole) {
+                const float inv = l[a] > 0.f ? 1.0f / l[a] : 0.f;
+                TT* dst = p.out + ((size_t)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh;
+#pragma unroll
+                for (int j = 0; j < 4 * NV; ++j) {
+                    const int col = tx * 4 + 64 * (j >> 2) + (j & 3);
+                    if (col < p.dh) bl_store(dst + col, o[a][j] * inv);
+                }
+            } else if (tx == 0) {
+                stats[2 * row] = m[a]; stats[2 * row + 1] = l[a];
+            }
+        }
+        if (!whole) {
 #pragma unroll
             for (int j = 0; j < 4 * NV; ++j) {
                 const int col = tx * 4 + 64 * (j >> 2) + (j & 3);
-                if (col < p.dh) {
-                    if (whole) bl_store(dst + col, o[a][j] * inv);
-                    else part[(size_t)row * p.dh + col] = o[a][j];
-                }
+                if (col < p.dh) *reinterpret_cast<float4*>(part + (size_t)col * ROWS + ty * 4) = make_float4(o[0][j], o[1][j], o[2][j], o[3][j]);
             }
-            if (!whole && tx == 0) { stats[2 * row] = m[a]; stats[2 * row + 1] = l[a]; }
         }
         left -= n_blocks;
         if (left > 0) tree_next_unit<KEYS>(p.line, w);
@@ -250,11 +252,9 @@ int launch(const Params<TT>& p, int blocks, cudaStream_t s) {
     }
     BL_CUDA(bl_launch_dependent(attention_tree_kernel<TT, VEC, NV>, dim3(blocks), dim3(THREADS), smem, s, p));
     BL_CHECK_LAUNCH("bl_attention_tree");
-    TreeMerge<TT> mg{p.line, p.scratch, p.out, blocks, p.dh, p.H, p.G};
-    if (blocks > 1) {
-        BL_CUDA(bl_launch_dependent(tree_merge_kernel<ROWS, KEYS, TT>, dim3(blocks - 1, ROWS / 8), dim3(256), 0, s, mg));
-        BL_CHECK_LAUNCH("bl_attention_tree (merge)");
-    }
+    TreeMerge<TT> mg{p.scratch, p.out, blocks, p.dh, p.H, p.G};
+    BL_CUDA(bl_launch_dependent(tree_merge_kernel<ROWS, 8 * NV, TT>, dim3(4 * bl_device_sms()), dim3(32 * TREE_MERGE_WARPS), 0, s, mg));
+    BL_CHECK_LAUNCH("bl_attention_tree (merge)");
     return 0;
 }
 
@@ -281,6 +281,8 @@ extern "C" int bl_attention_tree(const void* q, const void* k_cache, const void*
     if (!(scale > 0.f)) BL_FAIL("bl_attention_tree: the scale of the scores must be positive (got %g)", (double)scale);
     if (scratch == nullptr) BL_FAIL("bl_attention_tree: no scratch");
     const int G = H / KV, blocks = resident_blocks(dh), npt = ROWS / G < TREE_MAX_NODES ? ROWS / G : TREE_MAX_NODES;
+    if (!tree_line_fits(R, KV, npt, max_pages, page_size, KEYS) || blocks > TREE_MERGE_MAX)
+        BL_FAIL("bl_attention_tree: %d requests with tables of %d pages of %d tokens are more work than a launch counts", R, max_pages, page_size);
     const TreeLine line{cu_q, ctx_len, R, KV, window, npt};
     const auto* mk = reinterpret_cast<const unsigned long long*>(mask);
     const float scale_log2 = scale * 1.4426950408889634f;

@@ -5,14 +5,14 @@
 // shares the key/value head); its work is the blocks of KEYS keys that one of its rows may see. All units' blocks stand in one
 // line, request by request, and each block of the grid takes an equal, unbroken part of that line: a long request is spread over as many
 // blocks as it takes, short ones share a block, and no list has to be made on the host (a captured launch follows the
-// lengths that its buffers hold when it is replayed). A unit that lies inside one part is finished there; of a unit that is cut, every block
+// lengths that its buffers hold when it is replayed). A part that would begin or end up to SNAP key blocks from the edge of
+// a unit begins or ends there (a piece of a unit has its costs beside its key blocks: its queries, the pipeline's start, its outputs). A unit that lies inside one part is finished there; of a unit that is cut, every block
 // leaves its rows' unnormalised outputs, maxima and sums in the scratch, and a second, small launch merges them in the
 // order of the line.
 #pragma once
 #include "common.cuh"
 
 constexpr int TREE_MAX_NODES = 64;     // a node's view of its request's nodes is one 64-bit mask
-constexpr int TREE_MIN_BLOCKS = 2;     // no block takes fewer key blocks than this (of a line that has them)
 
 struct TreeLine {
     const int* cu_q; const int* ctx_len; int R, KV, window, npt;          // npt: nodes of a row tile
@@ -38,50 +38,6 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeLine& a, int r) {
 // A place of the line: key block b of unit (request r, key/value head kvh, tile).
 struct TreePlace { int r, kvh, tile, b; TreeRequest q; };
 
-template <int KEYS>
-__device__ __forceinline__ long long tree_blocks(const TreeLine& a, int r) {
-    if (r >= a.R) return 0;
-    const TreeRequest q = tree_request<KEYS>(a, r);
-    return (long long)q.tiles * a.KV * q.nb;
-}
-// All lanes of a warp: the length of the line.
-template <int KEYS>
-__device__ __forceinline__ long long tree_total(const TreeLine& a) {
-    long long sum = 0;
-    for (int r = threadIdx.x & 31; r < a.R; r += 32) sum += tree_blocks<KEYS>(a, r);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
-}
-// All lanes of a warp: where position `at` of the line lies (0 <= at < total).
-template <int KEYS>
-__device__ __forceinline__ TreePlace tree_find(const TreeLine& a, long long at) {
-    const int lane = threadIdx.x & 31;
-    TreePlace p{};
-    for (int r0 = 0; r0 < a.R; r0 += 32) {
-        const long long mine = tree_blocks<KEYS>(a, r0 + lane);
-        long long upto = mine;                                           // inclusive sum over the lanes
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned here = __ballot_sync(0xffffffffu, upto > at);
-        if (here) {
-            const int src = __ffs(here) - 1;
-            at -= __shfl_sync(0xffffffffu, upto - mine, src);
-            p.r = r0 + src;
-            break;
-        }
-        at -= __shfl_sync(0xffffffffu, upto, 31);
-    }
-    p.q = tree_request<KEYS>(a, p.r);
-    const int unit = (int)(at / p.q.nb);
-    p.b = p.q.b0 + (int)(at - (long long)unit * p.q.nb);
-    p.kvh = unit / p.q.tiles;
-    p.tile = unit - p.kvh * p.q.tiles;
-    return p;
-}
 // The first block of the unit behind p's (there is one).
 template <int KEYS>
 __device__ __forceinline__ void tree_next_unit(const TreeLine& a, TreePlace& p) {
@@ -94,11 +50,93 @@ __device__ __forceinline__ void tree_next_unit(const TreeLine& a, TreePlace& p) 
     }
     p.b = p.q.b0;
 }
-// How many blocks of the grid have a part of the line, and where the part of block i begins.
-__device__ __forceinline__ int tree_parts(long long total, int grid) {
-    return (int)max(1LL, min((long long)grid, total / TREE_MIN_BLOCKS));
+
+// A unit that the beginning of a part cuts, and no part before it: what the merge needs to know. parts = 0: there is none.
+struct TreeCut { int parts, first, slot, tok, nodes, kvh, pad0, pad1; };          // slots: first, then slot, slot + 2, .. (parts - 1 of them)
+// A block's part of the line: `left` key blocks from `place` on (0: none), and what there is to merge at its beginning.
+struct TreeShare { TreePlace place; int left; TreeCut cut; };
+
+// The share of block i of `grid`, by all lanes of a warp (the same answer in each). No part has fewer than MIN blocks (of a line that has
+// them). The line is shorter than 2^31 (the host sees to it). `ends`: 32 words of shared memory.
+template <int KEYS, int MIN, int SNAP>
+__device__ __forceinline__ TreeShare tree_share(const TreeLine& a, int grid, int i, int* ends) {
+    constexpr unsigned ALL = 0xffffffffu;
+    const int lane = threadIdx.x & 31, each = (a.R + 31) / 32;           // lane l adds up requests l * each ..
+    auto blocks = [&](const TreeRequest& q) { return q.tiles * a.KV * q.nb; };
+    int upto = 0;
+#pragma unroll 2
+    for (int r = lane * each; r < min(a.R, (lane + 1) * each); ++r) upto += blocks(tree_request<KEYS>(a, r));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(ALL, upto, o);
+        if (lane >= o) upto += up;
+    }
+    ends[lane] = upto;
+    __syncwarp();
+    const int total = __shfl_sync(ALL, upto, 31);
+    TreeShare s{};
+    if (total == 0) return s;
+    const int parts = max(1, min(grid, total / MIN)), per = total / parts, more = total - per * parts;
+    if (i >= parts) return s;
+    auto edge = [&](int k) { return per * k + min(k, more); };
+    // Lanes 0, 1 and 2 look up where parts i - 1, i and i + 1 begin, each by itself.
+    const int k = i - 1 + lane;
+    int at = k <= 0 ? 0 : total, begin = 0, length = 0;
+    TreePlace p{};
+    if (lane < 3 && k >= 0 && k < parts) {
+        at = edge(k);
+        int l = 0;
+#pragma unroll
+        for (int half = 16; half > 0; half >>= 1)
+            if (ends[l + half - 1] <= at) l += half;
+        int from = l > 0 ? ends[l - 1] : 0;
+        p.r = l * each;
+        p.q = tree_request<KEYS>(a, p.r);
+        while (from + blocks(p.q) <= at) {
+            from += blocks(p.q);
+            p.q = tree_request<KEYS>(a, ++p.r);
+        }
+        const int unit = (at - from) / p.q.nb;
+        length = p.q.nb;
+        begin = from + unit * length;
+        p.kvh = unit / p.q.tiles;
+        p.tile = unit - p.kvh * p.q.tiles;
+        if (SNAP > 0 && at - begin <= SNAP) at = begin;
+        if (SNAP > 0 && at > begin && begin + length - at <= SNAP) {
+            begin = at = begin + length;
+            if (at < total) tree_next_unit<KEYS>(a, p);
+            length = p.q.nb;
+        }
+        p.b = p.q.b0 + at - begin;
+    }
+    const int before = __shfl_sync(ALL, at, 0), start = __shfl_sync(ALL, at, 1), end = __shfl_sync(ALL, at, 2);
+    begin = __shfl_sync(ALL, begin, 1);
+    length = __shfl_sync(ALL, length, 1);
+    s.left = end - start;
+    if (s.left == 0) return s;
+    int* words = reinterpret_cast<int*>(&p);
+#pragma unroll
+    for (int x = 0; x < (int)(sizeof(TreePlace) / sizeof(int)); ++x) words[x] = __shfl_sync(ALL, words[x], 1);
+    s.place = p;
+    if (start > begin && before <= begin) {                              // parts i - 1, i, .. hold pieces of the unit
+        int inside = 0;
+        for (int x = i + lane; x < parts && edge(x) < begin + length - SNAP; x += 32) ++inside;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) inside += __shfl_xor_sync(ALL, inside, o);
+        s.cut.parts = 1 + inside;
+        s.cut.first = before == begin ? 2 * (i - 1) : 2 * (i - 1) + 1;
+        s.cut.slot = 2 * i;
+        s.cut.tok = p.q.begin + p.tile * a.npt;
+        s.cut.nodes = min(a.npt, p.q.n - p.tile * a.npt);
+        s.cut.kvh = p.kvh;
+    }
+    return s;
 }
-__device__ __forceinline__ long long tree_part(long long total, int parts, int i) { return total * i / parts; }
+// Whether the line is short enough for 32-bit places, whatever the lengths: every request with the most blocks that its table has room for.
+inline bool tree_line_fits(int R, int KV, int npt, int max_pages, int page_size, int keys) {
+    const long long tiles = (TREE_MAX_NODES + npt - 1) / npt, blocks = ((long long)max_pages * page_size + keys - 1) / keys + 1;
+    return (long long)R * KV * tiles <= 0x7fffffffLL / blocks;
+}
 
 // Which of the nodes a node sees: its mask without the bits of nodes that the request does not have and, with a window, without those
 // nodes further up than the window (on the way to a node the higher bit is the nearer node).
@@ -117,55 +155,102 @@ __device__ __forceinline__ unsigned tree_bits(unsigned long long mask, int c, in
     return w;
 }
 
-// The scratch: 2 * blocks slots of [rows][dh] outputs, then [2 * blocks][rows][2] maxima and sums. A block's first segment has slot
-// 2 * block, one that it begins (and the next block goes on with) slot 2 * block + 1.
-__host__ __device__ __forceinline__ size_t tree_scratch_floats(int blocks, int rows, int dh) { return (size_t)2 * blocks * rows * (dh + 2); }
+// The scratch: a TreeCut per block, then 2 * blocks slots of [dh][rows] outputs (a thread has a row: neighbouring threads write neighbouring
+// words), then [2 * blocks][rows][2] maxima and sums. A block's first segment has slot 2 * block, one that it begins (and the next
+// block goes on with) slot 2 * block + 1.
+__host__ __device__ __forceinline__ size_t tree_scratch_floats(int blocks, int rows, int dh) { return (size_t)8 * blocks + (size_t)2 * blocks * rows * (dh + 2); }
+__device__ __forceinline__ float* tree_outputs(float* scratch, int blocks) { return scratch + (size_t)8 * blocks; }
+__device__ __forceinline__ float* tree_stats(float* scratch, int blocks, int rows, int dh) { return scratch + (size_t)8 * blocks + (size_t)2 * blocks * rows * dh; }
 
 template <typename TT>
-struct TreeMerge { TreeLine line; const float* scratch; TT* out; int blocks, dh, H, G; };
+struct TreeMerge { float* scratch; TT* out; int blocks, dh, H, G; };
 
-// Block (i, y): the unit that the beginning of part i cuts, if no part before it does; a warp per row, rows y * warps .. of the tile.
-template <int ROWS, int KEYS, typename TT>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeMerge<TT> p) {
-    const int lane = threadIdx.x & 31;
+constexpr int TREE_MERGE_WARPS = 8, TREE_MERGE_MAX = 1024;               // most blocks of a launch whose units are merged
+constexpr int TREE_MERGE_MANY = 8;                                       // more parts than this: four blocks share 32 rows
+
+// o = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k over the parts k of each unit that is cut, in their order. The blocks share the rows of all
+// cut units out, 32 at a time: lane = row, a warp has NC columns (of a unit with many parts, as when one long request is on all SMs, NC
+// / 4 of them), and the finished rows leave through shared memory.
+template <int ROWS, int NC, typename TT>
+struct TreeMergeTile {
+    template <int COLS>
+    static __device__ __forceinline__ void run(const TreeMerge<TT>& p, const TreeCut& cut, int row0, int col_first, float* tile) {
+        constexpr int LD = TREE_MERGE_WARPS * COLS + 1;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = cut.nodes * p.G, row = row0 + lane, col0 = col_first + warp * COLS;
+        const float* outs = tree_outputs(p.scratch, p.blocks);
+        const float* stats = tree_stats(p.scratch, p.blocks, ROWS, p.dh);
+        const bool live = row < rows;
+        float m = -INFINITY, l = 0.f, o[COLS] = {};
+        constexpr int AHEAD = COLS <= 8 ? 4 : 2;                         // parts whose numbers are asked for together
+        for (int k0 = 0; k0 < cut.parts; k0 += AHEAD) {
+            float2 ml[AHEAD];
+            float v[AHEAD][COLS];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int k = k0 + u;
+                const bool there = live && k < cut.parts;
+                const size_t slot = k == 0 ? cut.first : cut.slot + 2 * (k - 1);
+                ml[u] = there ? *reinterpret_cast<const float2*>(stats + 2 * (slot * ROWS + row)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) v[u][j] = there && col0 + j < p.dh ? outs[(slot * p.dh + col0 + j) * ROWS + row] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {                            // one part more, against the larger of the two maxima
+                const float top = fmaxf(m, ml[u].x), use = top == -INFINITY ? 0.f : top;
+                const float a = exp2f(m - use), b = exp2f(ml[u].x - use);
+                m = top;
+                l = l * a + ml[u].y * b;
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) o[j] = o[j] * a + v[u][j] * b;
+            }
+        }
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) tile[lane * LD + warp * COLS + j] = o[j] * inv;
+        __syncthreads();
+        for (int x = tid; x < 32 * TREE_MERGE_WARPS * COLS; x += 32 * TREE_MERGE_WARPS) {
+            const int r = x / (TREE_MERGE_WARPS * COLS), c = x - r * (TREE_MERGE_WARPS * COLS), node = (row0 + r) / p.G;
+            if (row0 + r < rows && col_first + c < p.dh)
+                bl_store(p.out + ((size_t)(cut.tok + node) * p.H + cut.kvh * p.G + row0 + r - node * p.G) * p.dh + col_first + c, tile[r * LD + c]);
+        }
+        __syncthreads();
+    }
+};
+
+template <int ROWS, int NC, typename TT>
+__global__ void __launch_bounds__(32 * TREE_MERGE_WARPS) tree_merge_kernel(const TreeMerge<TT> p) {
+    __shared__ float tile[32 * (TREE_MERGE_WARPS * NC + 1)];
+    __shared__ int upto[TREE_MERGE_MAX], warp_sum[TREE_MERGE_WARPS];     // items of the cuts up to each
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     bl_pdl_wait();
     bl_pdl_trigger();
-    const long long total = tree_total<KEYS>(p.line);
-    if (total == 0) return;
-    const int parts = tree_parts(total, p.blocks), i = blockIdx.x + 1;
-    if (i >= parts) return;
-    const long long at = tree_part(total, parts, i);
-    const TreePlace u = tree_find<KEYS>(p.line, at);
-    const long long begin = at - (u.b - u.q.b0), end = begin + u.q.nb;
-    if (at == begin || tree_part(total, parts, i - 1) > begin) return;   // not cut here, or cut before
-    const int row = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int nodes = min(p.line.npt, u.q.n - u.tile * p.line.npt);
-    if (row >= nodes * p.G) return;
-    const int first = tree_part(total, parts, i - 1) == begin ? 2 * (i - 1) : 2 * (i - 1) + 1;
-    const float* stats = p.scratch + (size_t)2 * p.blocks * ROWS * p.dh;
-    int last = i;                                                        // parts i - 1 .. last hold the unit
-    while (last + 1 < parts && tree_part(total, parts, last + 1) < end) ++last;
-    float m = -INFINITY;
-    for (int k = i - 1 + lane; k <= last; k += 32) m = fmaxf(m, stats[2 * ((size_t)(k < i ? first : 2 * k) * ROWS + row)]);
-    m = bl_warp_max(m);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[8];
+    const TreeCut* cuts = reinterpret_cast<const TreeCut*>(p.scratch);
+    auto items_of = [&](int parts, int nodes) { return parts == 0 ? 0 : (nodes * p.G + 31) / 32 * (parts > TREE_MERGE_MANY ? 4 : 1); };
+    int total = 0;
+    for (int i0 = 0; i0 < p.blocks; i0 += 32 * TREE_MERGE_WARPS) {
+        int mine = i0 + tid < p.blocks ? items_of(cuts[i0 + tid].parts, cuts[i0 + tid].nodes) : 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = 0.f;
-#pragma unroll 4
-    for (int k = i - 1; k <= last; ++k) {
-        const size_t slot = (size_t)(k < i ? first : 2 * k) * ROWS + row;
-        const float2 ml = *reinterpret_cast<const float2*>(stats + 2 * slot);
-        const float w = exp2f(ml.x - m_use);
-        l = fmaf(w, ml.y, l);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < p.dh) o[j] = fmaf(w, p.scratch[slot * p.dh + lane + 32 * j], o[j]);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += v;
+        }
+        if (lane == 31) warp_sum[warp] = mine;
+        __syncthreads();
+        int before = total;
+        for (int w = 0; w < TREE_MERGE_WARPS; ++w) {
+            if (w < warp) before += warp_sum[w];
+            total += warp_sum[w];
+        }
+        if (i0 + tid < p.blocks) upto[i0 + tid] = before + mine;
+        __syncthreads();
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const int node = row / p.G, head = u.kvh * p.G + row - node * p.G;
-    TT* dst = p.out + ((size_t)(u.q.begin + u.tile * p.line.npt + node) * p.H + head) * p.dh;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < p.dh) bl_store(dst + lane + 32 * j, o[j] * inv);
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        int at = 0;                                                      // the first cut whose items reach beyond this one
+        for (int half = TREE_MERGE_MAX / 2; half > 0; half >>= 1)
+            if (at + half <= p.blocks && upto[at + half - 1] <= item) at += half;
+        const TreeCut cut = cuts[at];
+        const int nth = item - (upto[at] - items_of(cut.parts, cut.nodes));
+        if (cut.parts > TREE_MERGE_MANY) TreeMergeTile<ROWS, NC, TT>::template run<NC / 4>(p, cut, nth / 4 * 32, nth % 4 * (TREE_MERGE_WARPS * NC / 4), tile);
+        else TreeMergeTile<ROWS, NC, TT>::template run<NC>(p, cut, nth * 32, 0, tile);
+    }
 }

@@ -91,37 +91,56 @@ def test_copy_blocks_c_entry_refuses(pairs, what):
     assert "more than the 8" in lib.bl_last_error().decode()
 
 
+@pytest.mark.parametrize("least,snap", [(1, 0), (4, 2)])
 @pytest.mark.parametrize("grid", [1, 3, 148, 296])
-def test_the_line_of_work_is_shared_out_whole(grid):
-    """attention_tree.cuh restated: for units of any lengths, the parts cover the line once, at most two segments of a part are
-    cut, and the merge of a unit starts at exactly one boundary."""
+def test_the_line_of_work_is_shared_out_whole(grid, least, snap):
+    """attention_tree.cuh restated: for units of any lengths, the parts cover the line once, no piece of a cut unit is as short as
+    the distance at which parts snap to its edges, every piece has a slot of its own, and each cut unit is merged once, from all of its pieces in their order."""
     rng = np.random.default_rng(grid)
-    for _ in range(60):
-        units = rng.integers(1, 60, int(rng.integers(1, 40))).tolist()
+    for trial in range(120):
+        units = rng.integers(1, [8, 60, 400][trial % 3], int(rng.integers(1, 40))).tolist()
         begins = np.concatenate([[0], np.cumsum(units)])
         total = int(begins[-1])
-        parts = max(1, min(grid, total // 2))
-        part = [total * i // parts for i in range(parts + 1)]
+        parts = max(1, min(grid, total // least))
+        per, more = total // parts, total % parts
+        edge = lambda k: per * k + min(k, more)
+
+        def unit_of(x):
+            u = int(np.searchsorted(begins, x, side="right")) - 1
+            return u, int(begins[u]), units[u]
+
+        def snapped(k):
+            if k <= 0:
+                return 0
+            if k >= parts or edge(k) >= total:
+                return total
+            x = edge(k)
+            _, begin, length = unit_of(x)
+            return begin if x - begin <= snap else begin + length if begin + length - x <= snap else x
+
         slots, merged = {}, []
         for i in range(parts):
-            at, first = part[i], True
-            while at < part[i + 1]:
-                u = int(np.searchsorted(begins, at, side="right")) - 1
-                n = min(part[i + 1] - at, int(begins[u + 1]) - at)
-                if n != units[u]:
+            at, end, first = snapped(i), snapped(i + 1), True
+            assert at <= end
+            while at < end:
+                u, begin, length = unit_of(at)
+                n = min(end, begin + length) - at
+                if n != length:
+                    assert n > snap
                     slot = 2 * i + (0 if first else 1)
                     assert slot not in slots
                     slots[slot] = u
                 at, first = at + n, False
+        assert snapped(0) == 0 and snapped(parts) == total
         for i in range(1, parts):
-            u = int(np.searchsorted(begins, part[i], side="right")) - 1
-            begin, end = int(begins[u]), int(begins[u + 1])
-            if part[i] == begin or part[i - 1] > begin:
+            start, before = snapped(i), snapped(i - 1)
+            if snapped(i + 1) == start:
                 continue
-            last = i
-            while last + 1 < parts and part[last + 1] < end:
-                last += 1
-            first = 2 * (i - 1) if part[i - 1] == begin else 2 * (i - 1) + 1
-            assert [first] + [2 * k for k in range(i, last + 1)] == sorted(s for s, unit in slots.items() if unit == u)
+            u, begin, length = unit_of(start)
+            if start == begin or before > begin:
+                continue
+            inside = sum(1 for k in range(i, parts) if edge(k) < begin + length - snap)
+            first = 2 * (i - 1) if before == begin else 2 * (i - 1) + 1
+            assert [first] + [2 * k for k in range(i, i + inside)] == sorted(s for s, unit in slots.items() if unit == u)
             merged.append(u)
         assert sorted(merged) == sorted(set(slots.values()))
