@@ -630,14 +630,13 @@ int bl_attention_tree_tc_status(int* status);
 // parent. The deepest accepted node (the lowest of several) ends the path: counts[r] nodes, path[r, 0..63] (then -1), answer[r, j] =
 // sampled[path[r, j]] (then -1). Node j of the path moves from cache row c + path[j] to c + j in all layers; k_pages and v_pages are
 // [layers][pages, KV, page_size, dh], the layers *_layer_stride elements apart.
-// bl_copy_blocks: t[layer, pairs[i][1]] = t[layer, pairs[i][0]] for tensors of `blocks` blocks of block_bytes bytes in layers that are
-// layer_bytes apart; `pairs` (and the other lists) lie in host memory and are read during the call. No target twice, none that is a source.
+// bl_copy_blocks: t[layer, pairs[i][1]] = t[layer, pairs[i][0]]; `tensors` [n_tensors][5]: address, bytes from layer to layer, bytes of a
+// block, layers, blocks of a layer. Both lists lie in host memory and are read during the call. No target twice, none that is a source.
 int bl_accept_tree(const int* sampled, const int* tokens, const long long* mask, const int* cu_q, const int* ctx_len,
                    const int* block_table, int max_pages, void* k_pages, void* v_pages, int elem_bytes, long long k_layer_stride,
                    long long v_layer_stride, int layers, int KV, int page_size, int dh, int* counts, int* path, int* answer, int R,
                    void* stream);
-int bl_copy_blocks(int n_tensors, void* const* bases, const long long* layer_bytes, const long long* block_bytes, const int* layers,
-                   const int* blocks, const int* pairs, int n_pairs, void* stream);
+int bl_copy_blocks(int n_tensors, const long long* tensors, const int* pairs, int n_pairs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) accept_tree_kernel(const Accept p) {
 // stores. The pairs stand in the launch's parameters: no list has to reach the device first.
 constexpr int MAX_TENSORS = 8, CHUNK = 16 * 1024, COPY_THREADS = 256;
 
-struct CopyTensor { char* base; long long layer, block, bytes; int first; };   // first: of its (layer, pair) items in the grid
+struct CopyTensor { char* base; long long layer, block, bytes; int first, layers; };   // first: of its (layer, pair) items in the grid
 template <int N> struct CopyList { CopyTensor t[MAX_TENSORS]; int tensors, pairs; int pair[2 * N]; };
 
 template <typename P, int N>
@@ -152,15 +152,18 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_blocks_kernel(const __grid_
 }
 
 template <int N>
-int launch_copies(CopyList<N>& list, const int* layers, const int* pairs, int n_pairs, int unit, cudaStream_t s) {
+int launch_copies(const CopyTensor* tensors, int n_tensors, const int* pairs, int n_pairs, int unit, cudaStream_t s) {
+    CopyList<N> list;
+    list.tensors = n_tensors;
+    memcpy(list.t, tensors, sizeof(CopyTensor) * n_tensors);
     for (int p0 = 0; p0 < n_pairs; p0 += N) {
         list.pairs = n_pairs - p0 < N ? n_pairs - p0 : N;
         memcpy(list.pair, pairs + 2 * p0, sizeof(int) * 2 * list.pairs);
         long long items = 0, most = 1;
         for (int t = 0; t < list.tensors; ++t) {
-            if (items + (long long)layers[t] * list.pairs > 2147483647LL) BL_FAIL("bl_copy_blocks: more copies than a launch takes");
+            if (items + (long long)list.t[t].layers * list.pairs > 2147483647LL) BL_FAIL("bl_copy_blocks: more copies than a launch takes");
             list.t[t].first = (int)items;
-            items += (long long)layers[t] * list.pairs;
+            items += (long long)list.t[t].layers * list.pairs;
             if (list.t[t].bytes > most) most = list.t[t].bytes;
         }
         if (items == 0) return 0;
@@ -221,23 +224,21 @@ extern "C" int bl_accept_tree(const int* sampled, const int* tokens, const long 
     return 0;
 }
 
-extern "C" int bl_copy_blocks(int n_tensors, void* const* bases, const long long* layer_bytes, const long long* block_bytes, const int* layers,
-                              const int* blocks, const int* pairs, int n_pairs, void* stream) {
+extern "C" int bl_copy_blocks(int n_tensors, const long long* tensors, const int* pairs, int n_pairs, void* stream) {
     if (n_tensors < 0 || n_pairs < 0) BL_FAIL("bl_copy_blocks: bad sizes");
     if (n_tensors == 0 || n_pairs == 0) return 0;
     if (n_tensors > MAX_TENSORS) BL_FAIL("bl_copy_blocks: %d tensors are more than the %d of a launch", n_tensors, MAX_TENSORS);
-    long long fewest = blocks[0], all = 0;
-    for (int t = 0; t < n_tensors; ++t) {
-        if (blocks[t] < fewest) fewest = blocks[t];
-        all |= (long long)(uintptr_t)bases[t] | layer_bytes[t] | block_bytes[t];
+    long long fewest = tensors[4], all = 0;
+    CopyTensor t[MAX_TENSORS];
+    for (int i = 0; i < n_tensors; ++i) {
+        const long long* x = tensors + 5 * i;
+        if (x[2] < 0 || x[3] < 0 || x[3] > 0x7fffffffLL || x[4] < 0 || x[4] > 0x7fffffffLL) BL_FAIL("bl_copy_blocks: bad sizes of tensor %d", i);
+        if (x[4] < fewest) fewest = x[4];
+        all |= x[0] | x[1] | x[2];
+        t[i] = CopyTensor{(char*)x[0], x[1], x[2], x[2], 0, (int)x[3]};
     }
     if (check_pairs(pairs, n_pairs, fewest)) return 1;
     const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-    const auto fill = [&](CopyTensor* t) { for (int i = 0; i < n_tensors; ++i) t[i] = CopyTensor{(char*)bases[i], layer_bytes[i], block_bytes[i], block_bytes[i], 0}; };
-    if (n_pairs <= 32) {
-        CopyList<32> list; list.tensors = n_tensors; fill(list.t);
-        return launch_copies(list, layers, pairs, n_pairs, unit, (cudaStream_t)stream);
-    }
-    CopyList<1024> list; list.tensors = n_tensors; fill(list.t);
-    return launch_copies(list, layers, pairs, n_pairs, unit, (cudaStream_t)stream);
+    if (n_pairs <= 32) return launch_copies<32>(t, n_tensors, pairs, n_pairs, unit, (cudaStream_t)stream);
+    return launch_copies<1024>(t, n_tensors, pairs, n_pairs, unit, (cudaStream_t)stream);
 }

@@ -2181,23 +2181,39 @@ TREE_MAX_NODES = 64       # nodes of one request in a step: what a node sees of 
 
 def _here(*tensors: torch.Tensor) -> None:
     """All on the current CUDA device, whose current stream the kernels are launched on."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise KernelError("must be CUDA tensors")
-    now = torch.cuda.current_device()
-    for t in tensors:
-        if t.device.index != now:
-            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{now}")
+    devices = {t.get_device() for t in tensors}
+    if -1 in devices:
+        raise KernelError("must be CUDA tensors")
+    now = torch.cuda.current_device() if _raw_device is None else _raw_device()
+    if devices != {now}:
+        raise KernelError(f"tensors lie on devices {sorted(devices)}, the current device is {now}")
 
 
 def _fits(t: torch.Tensor, name: str, dtype, shape) -> None:
     """The part of `_need` that needs no device."""
-    if t.dtype != dtype:
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return
+    if t.dtype is not dtype:
         raise KernelError(f"{name}: must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise KernelError(f"{name}: must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise KernelError(f"{name}: must be contiguous")
+    raise KernelError(f"{name}: must be contiguous")
+
+
+_LL = ctypes.c_longlong
+_TYPED = {
+    # entry points that are called with plain numbers: with their types declared a call costs a third of what it does with a
+    # ctypes object for each pointer (these operators stand between short launches)
+    "bl_attention_tree": "pppipppp" "ipp" "iiiiiii" "fp", "bl_attention_tree_tc": "ppppppp" "ipp" "iiiiiiii" "fp",
+    "bl_accept_tree": "pppppp" "ippi" "qqiiiipppip", "bl_copy_blocks": "ippip"}
+
+
+@functools.lru_cache(maxsize=None)
+def _typed(name: str):
+    fn = getattr(_lib(), name)
+    kinds = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": _LL, "f": ctypes.c_float}
+    fn.argtypes = [kinds[k] for k in _TYPED[name]]
+    return fn
 
 
 def _tree_step(mask: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor):
@@ -2206,7 +2222,8 @@ def _tree_step(mask: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor, bl
     _fits(mask, "mask", torch.int64, (T,)); _fits(cu_q, "cu_q", torch.int32, (R + 1,)); _fits(ctx_len, "ctx_len", torch.int32, (R,))
     if block_table.dim() != 2 or block_table.shape[0] < R:
         raise KernelError(f"block_table: must have a row for each of the {R} requests, got {tuple(block_table.shape)}")
-    _fits(block_table, "block_table", torch.int32, block_table.shape)
+    if block_table.dtype is not torch.int32 or not block_table.is_contiguous():
+        raise KernelError("block_table: must be contiguous int32")
     if T > TREE_MAX_NODES * R:
         raise KernelError(f"{T} nodes are more than {TREE_MAX_NODES} for each of {R} requests")
     return T, R
@@ -2231,22 +2248,14 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _fits(q, "q", q.dtype, (T, H * dh)); _fits(k_cache, "k_cache", q.dtype, k_cache.shape)
     _fits(v_cache, "v_cache", q.dtype, k_cache.shape); _fits(out, "out", q.dtype, (T, H * dh))
     _here(q, k_cache, v_cache, cu_q, ctx_len, mask, block_table, out)
-    lib = _lib()
-    if attention_tree_tc_supported(q, k_cache, v_cache, out, H):
-        scratch = torch.empty(_tree_scratch(dh, True), dtype=torch.float32, device=q.device)
-        _call(lib.bl_attention_tree_tc, _p(q), _p(k_cache), _p(v_cache), _p(cu_q), _p(ctx_len), _p(mask), _p(block_table), block_table.shape[1],
-              _p(out), _p(scratch), T, R, k_cache.shape[0], H, KV, dh, page_size, window, ctypes.c_float(scale), _stream())
-        return
-    scratch = torch.empty(_tree_scratch(dh, False), dtype=torch.float32, device=q.device)
-    _call(lib.bl_attention_tree, _p(q), _p(k_cache), _p(v_cache), _dt(q), _p(cu_q), _p(ctx_len), _p(mask), _p(block_table),
-          block_table.shape[1], _p(out), _p(scratch), T, R, H, KV, dh, page_size, window, ctypes.c_float(scale), _stream())
-
-
-def attention_tree_tc_supported(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, H: int) -> bool:
-    """Whether `attention_tree` runs these operands on the tensor cores: bfloat16, 16-byte aligned, head size 64 or 128, pages of 16."""
-    _, KV, page_size, dh = k_cache.shape
-    return (q.dtype == torch.bfloat16 and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
-            and _tree_tc_built(H, KV, dh, page_size))
+    ptr_q, ptr_k, ptr_v, ptr_out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    tc = q.dtype is torch.bfloat16 and (ptr_q | ptr_k | ptr_v | ptr_out) % 16 == 0 and _tree_tc_built(H, KV, dh, page_size)
+    scratch = torch.empty(_tree_scratch(dh, tc), dtype=torch.float32, device=q.device)
+    rest = (cu_q.data_ptr(), ctx_len.data_ptr(), mask.data_ptr(), block_table.data_ptr(), block_table.shape[1], ptr_out, scratch.data_ptr(), T, R)
+    if tc:
+        _call(_typed("bl_attention_tree_tc"), ptr_q, ptr_k, ptr_v, *rest, k_cache.shape[0], H, KV, dh, page_size, window, scale, _stream().value)
+    else:
+        _call(_typed("bl_attention_tree"), ptr_q, ptr_k, ptr_v, _dt(q), *rest, H, KV, dh, page_size, window, scale, _stream().value)
 
 
 @functools.lru_cache(maxsize=None)
@@ -2270,25 +2279,25 @@ def accept_tree(sampled: torch.Tensor, token_ids: torch.Tensor, mask: torch.Tens
     ancestors are and its token is the one sampled behind its parent. The deepest accepted node, the lowest of several, ends the path:
     `counts` nodes, `path` their numbers (then -1), `tokens` what is sampled behind them (then -1). The path's keys and values move to
     cache rows c, c + 1, .. of `k_pages` and `v_pages` [layers, pages, kv heads, page size, head size] (contiguous layers), in place; the pages
-    that hold a request's nodes must be its own. The three results are views of one buffer, counts and tokens first."""
+    that hold a request's nodes must be its own."""
     T, R = _tree_step(mask, cu_q, ctx_len, block_table)
     _fits(sampled, "sampled", torch.int32, (T,)); _fits(token_ids, "token_ids", torch.int32, (T,))
     if k_pages.dim() != 5 or k_pages.shape != v_pages.shape:
         raise KernelError(f"k_pages, v_pages: must be [layers, pages, kv heads, page size, head size] alike, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     layers, pages, KV, page_size, dh = k_pages.shape
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _dt(t)
-        if t.dtype != k_pages.dtype or t.stride()[1:] != (KV * page_size * dh, page_size * dh, dh, 1) or t.stride(0) < pages * KV * page_size * dh:
-            raise KernelError(f"{name}: each layer must be contiguous, layers must not overlap, and the dtypes must agree")
+    _dt(k_pages)
+    rows, k_stride, v_stride = (KV * page_size * dh, page_size * dh, dh, 1), k_pages.stride(), v_pages.stride()
+    least = pages * rows[0] if layers > 1 else 0
+    if v_pages.dtype is not k_pages.dtype or k_stride[1:] != rows or v_stride[1:] != rows or k_stride[0] < least or v_stride[0] < least:
+        raise KernelError("k_pages, v_pages: each layer must be contiguous, layers must not overlap, and the dtypes must agree")
     _here(sampled, token_ids, mask, cu_q, ctx_len, k_pages, v_pages, block_table)
-    lib = _lib()
-    got = torch.empty((1 + 2 * TREE_MAX_NODES) * R, dtype=torch.int32, device=mask.device)
-    tokens, path = got[R:(1 + TREE_MAX_NODES) * R].view(R, TREE_MAX_NODES), got[(1 + TREE_MAX_NODES) * R:].view(R, TREE_MAX_NODES)
-    LL = ctypes.c_longlong
-    _call(lib.bl_accept_tree, _p(sampled), _p(token_ids), _p(mask), _p(cu_q), _p(ctx_len), _p(block_table), block_table.shape[1],
-          _p(k_pages), _p(v_pages), k_pages.element_size(), LL(k_pages.stride(0)), LL(v_pages.stride(0)), layers, KV, page_size, dh, _p(got),
-          _p(path), _p(tokens), R, _stream())
-    return got[:R], path, tokens
+    device = mask.device
+    counts = torch.empty(R, dtype=torch.int32, device=device)
+    path, tokens = (torch.empty((R, TREE_MAX_NODES), dtype=torch.int32, device=device) for _ in range(2))
+    _call(_typed("bl_accept_tree"), sampled.data_ptr(), token_ids.data_ptr(), mask.data_ptr(), cu_q.data_ptr(), ctx_len.data_ptr(),
+          block_table.data_ptr(), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.element_size(), k_stride[0],
+          v_stride[0], layers, KV, page_size, dh, counts.data_ptr(), path.data_ptr(), tokens.data_ptr(), R, _stream().value)
+    return counts, path, tokens
 
 
 def copy_blocks(tensors, pairs) -> None:
@@ -2298,25 +2307,27 @@ def copy_blocks(tensors, pairs) -> None:
     flat = array.array("i", itertools.chain.from_iterable(pairs))
     if len(flat) != 2 * len(pairs):
         raise KernelError("pairs: must be pairs of block numbers")
-    n = len(tensors)
-    bases, layer_bytes, block_bytes = (ctypes.c_void_p * n)(), (ctypes.c_longlong * n)(), (ctypes.c_longlong * n)()
-    layers, blocks = (ctypes.c_int * n)(), (ctypes.c_int * n)()
+    lists = array.array("q")
     for i, t in enumerate(tensors):
-        if t.dim() < 2:
-            raise KernelError(f"tensor {i}: must be [layers, blocks, ...], got {tuple(t.shape)}")
-        size = 1
-        for extent, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if extent != 1 and stride != size:
-                raise KernelError(f"tensor {i}: the blocks of a layer must be contiguous")
-            size *= extent
-        if t.shape[0] > 1 and t.stride(0) < size:
-            raise KernelError(f"tensor {i}: layers must not overlap")
+        layers, blocks, layer_items, block_items = _block_layout(t.shape, t.stride(), i)
         item = t.element_size()
-        bases[i], layer_bytes[i] = t.data_ptr(), t.stride(0) * item
-        layers[i], blocks[i] = t.shape[0], t.shape[1]
-        block_bytes[i] = size // max(1, t.shape[1]) * item
-    if n == 0 or len(flat) == 0:
+        lists.extend((t.data_ptr(), layer_items * item, block_items * item, layers, blocks))
+    if len(tensors) == 0 or len(flat) == 0:
         return
     _here(*tensors)
-    at, _ = flat.buffer_info()
-    _call(_lib().bl_copy_blocks, n, bases, layer_bytes, block_bytes, layers, blocks, ctypes.c_void_p(at), len(pairs), _stream())
+    _call(_typed("bl_copy_blocks"), len(tensors), lists.buffer_info()[0], flat.buffer_info()[0], len(pairs), _stream().value)
+
+
+@functools.lru_cache(maxsize=256)
+def _block_layout(shape, stride, i: int):
+    """(layers, blocks, items from layer to layer, items of a block) of a tensor [layers, blocks, ...]."""
+    if len(shape) < 2:
+        raise KernelError(f"tensor {i}: must be [layers, blocks, ...], got {tuple(shape)}")
+    size = 1
+    for n, step in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if n != 1 and step != size:
+            raise KernelError(f"tensor {i}: the blocks of a layer must be contiguous")
+        size *= n
+    if shape[0] > 1 and stride[0] < size:
+        raise KernelError(f"tensor {i}: layers must not overlap")
+    return shape[0], shape[1], stride[0], size // max(1, shape[1])

@@ -81,13 +81,13 @@ def test_copy_blocks_refuses(tensors, pairs, what):
 @pytest.mark.parametrize("pairs,what", [([(0, 5)], "outside"), ([(-1, 2)], "outside"), ([(5, 2)], "outside"), ([(0, 2), (1, 2)], "target of two"),
                                         ([(0, 2), (2, 3)], "both source and target"), ([(1, 1)], "both source and target")])
 def test_copy_blocks_c_entry_refuses(pairs, what):
-    one = (ctypes.c_longlong * 1)(64)
     flat = array.array("i", [x for p in pairs for x in p])
     lib = library.load()
-    bases, counts, blocks = (ctypes.c_void_p * 1)(4096), (ctypes.c_int * 1)(1), (ctypes.c_int * 1)(5)
-    assert lib.bl_copy_blocks(1, bases, one, one, counts, blocks, ctypes.c_void_p(flat.buffer_info()[0]), len(pairs), ctypes.c_void_p(0)) == 1
+    tensors = array.array("q", [4096, 64, 64, 1, 5] * 9)
+    at = lambda a: ctypes.c_void_p(a.buffer_info()[0])
+    assert lib.bl_copy_blocks(1, at(tensors), at(flat), len(pairs), ctypes.c_void_p(0)) == 1
     assert what in lib.bl_last_error().decode()
-    assert lib.bl_copy_blocks(9, bases, one, one, counts, blocks, ctypes.c_void_p(flat.buffer_info()[0]), 1, ctypes.c_void_p(0)) == 1
+    assert lib.bl_copy_blocks(9, at(tensors), at(flat), 1, ctypes.c_void_p(0)) == 1
     assert "more than the 8" in lib.bl_last_error().decode()
 
 
