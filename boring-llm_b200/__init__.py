@@ -12,7 +12,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # the engine needs torch.cuda; import it only when asked for
-    if name in ("Engine", "generate", "SamplingParams", "Request", "ModelRunner", "StepEntry", "Scheduler"):
+    if name in ("Engine", "generate", "SamplingParams", "Request", "ModelRunner", "StepEntry", "TreeEntry", "Scheduler"):
         from . import engine as _engine
         return getattr(_engine, name)
     raise AttributeError(name)

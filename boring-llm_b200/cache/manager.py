@@ -69,6 +69,7 @@ class PagePool:
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self._owner: List[Optional[object]] = [None] * num_pages
+        self._others: Dict[int, List[object]] = {}     # page -> its further owners (requests that were forked share pages)
         self.high_water = 0
         self.freed_log: Optional[List[int]] = None     # when a list: every page given back is noted here (debugging)
 
@@ -91,6 +92,15 @@ class PagePool:
             raise CacheError(f"page {page} is outside the pool")
         if self._owner[page] is None:
             raise CacheError(f"page {page} freed twice")
+        others = self._others.get(page)
+        if others and (self._owner[page] == owner or owner in others):
+            if self._owner[page] == owner:             # the page stays with the others
+                self._owner[page] = others.pop(0)
+            else:
+                others.remove(owner)
+            if not others:
+                del self._others[page]
+            return
         if self._owner[page] != owner:
             raise CacheError(f"page {page} is owned by {self._owner[page]!r}, not by {owner!r}")
         self._owner[page] = None
@@ -100,6 +110,20 @@ class PagePool:
 
     def owner_of(self, page: int):
         return self._owner[page]
+
+    def share(self, page: int, owner) -> None:
+        """One more owner of a page that is held."""
+        if self._owner[page] is None:
+            raise CacheError(f"page {page} is free and cannot be shared")
+        if owner in self.owners_of(page):
+            raise CacheError(f"page {page} is held by {owner!r} already")
+        self._others.setdefault(page, []).append(owner)
+
+    def is_shared(self, page: int) -> bool:
+        return page in self._others
+
+    def owners_of(self, page: int) -> List[object]:
+        return ([] if self._owner[page] is None else [self._owner[page]]) + self._others.get(page, [])
 
 
 @dataclass
@@ -125,6 +149,7 @@ class RequestCache:
     tables: List[List[int]] = field(default_factory=list)
     uid: int = 0          # unlike request_id never used twice by one manager
     version: int = 0      # counts the changes of `tables`: (uid, version) names one state of the block tables
+    forked: bool = False  # this request may share pages with others: the one that it writes next has to be looked at
 
 
 class CacheManager:
@@ -173,6 +198,8 @@ class CacheManager:
         self._requests: Dict[object, RequestCache] = {}
         self._on_slot_assigned = on_slot_assigned
         self._next_uid = 0
+        # per paged group: (page, its copy) pairs that have to be copied before the next step writes (`take_copies`)
+        self._copies: List[List[Tuple[int, int]]] = [[] for _ in self.paged_groups]
 
     # ---- requests -------------------------------------------------------------------------
     def has_free_slot(self) -> bool:
@@ -210,7 +237,16 @@ class CacheManager:
     # ---- pages ----------------------------------------------------------------------------
     def _pages_needed(self, rc: RequestCache, n_new: int) -> List[int]:
         total = -(-(rc.num_tokens + n_new) // self.page_size)
-        return [max(0, total - len(t)) for t in rc.tables]
+        return [max(0, total - len(t)) + (1 if rc.forked and self._writes_shared(rc, g, t) else 0) for g, t in zip(self.paged_groups, rc.tables)]
+
+    def _writes_shared(self, rc: RequestCache, group: PagedGroup, table: List[int]) -> bool:
+        """Whether the page that the request's next token goes to is one that other requests hold, too."""
+        at = rc.num_tokens // self.page_size
+        return rc.num_tokens % self.page_size != 0 and at < len(table) and table[at] >= 0 and group.pool.is_shared(table[at])
+
+    def pages_needed(self, request_id, n_new: int) -> List[int]:
+        """Pages that `n_new` more tokens take from each group's pool (the copy of a shared page among them)."""
+        return self._pages_needed(self.get(request_id), n_new)
 
     def can_reserve(self, request_id, n_new: int) -> bool:
         rc = self.get(request_id)
@@ -231,12 +267,56 @@ class CacheManager:
         need = self._pages_needed(rc, n_new)
         if any(n > g.pool.num_free for n, g in zip(need, self.paged_groups)):
             return False
-        for n, g, table in zip(need, self.paged_groups, rc.tables):
+        for gi, (n, g, table) in enumerate(zip(need, self.paged_groups, rc.tables)):
+            if n and rc.forked and self._writes_shared(rc, g, table):
+                # the next token goes to a page that others read: this request goes on in a copy of its own
+                at, page = rc.num_tokens // self.page_size, g.pool.take(request_id)
+                self._copies[gi].append((table[at], page))
+                g.pool.give_back(table[at], request_id)
+                table[at] = page
+                rc.version += 1
+                n -= 1
             for _ in range(n):
                 table.append(g.pool.take(request_id))
             if n:
                 rc.version += 1
         return True
+
+    def fork(self, request_id, new_id, n_keep: Optional[int] = None) -> RequestCache:
+        """A new request that holds the first `n_keep` tokens (default: all) of a live one: it shares their pages, and whoever
+        writes to a shared page first goes on in a copy (`reserve`; the storage copies what `take_copies` returns before the
+        next step). Costs no pages now. The caller copies the state slot, if there are state groups (then `n_keep` must be all). Not
+        possible once a window has given pages back that the shorter prefix needs."""
+        rc = self.get(request_id)
+        n_keep = rc.num_tokens if n_keep is None else n_keep
+        if not 0 <= n_keep <= rc.num_tokens:
+            raise CacheError(f"fork: {n_keep} tokens outside 0..{rc.num_tokens}")
+        if self.state_groups and n_keep != rc.num_tokens:
+            raise CacheError("fork: state of fixed size holds all of a request's tokens, not a prefix")
+        keep_pages = -(-n_keep // self.page_size)
+        for g, table in zip(self.paged_groups, rc.tables):
+            first = max(0, g.spec.first_needed(n_keep)) // self.page_size
+            if any(p < 0 for p in table[first:keep_pages]):
+                raise CacheError("fork: a window has already given pages of the kept prefix back")
+        new = self.add_request(new_id)
+        new.num_tokens = n_keep
+        for g, table, into in zip(self.paged_groups, rc.tables, new.tables):
+            for p in table[:keep_pages]:
+                if p >= 0:
+                    g.pool.share(p, new_id)
+                into.append(p)
+        rc.forked = new.forked = True
+        new.version += 1
+        return new
+
+    def take_copies(self) -> List[List[Tuple[int, int]]]:
+        """Per paged group the (page, copy) pairs that have come up since the last call, each copy once."""
+        out, self._copies = self._copies, [[] for _ in self.paged_groups]
+        return out
+
+    @property
+    def has_copies(self) -> bool:
+        return any(self._copies)
 
     def commit(self, request_id, n_new: int) -> None:
         """The step has written `n_new` tokens. Pages that every later query's window has passed
@@ -303,16 +383,20 @@ class CacheManager:
     def check(self) -> None:
         """No page lost, held twice or both free and held; slots likewise. Raises CacheError."""
         for gi, g in enumerate(self.paged_groups):
-            held: Dict[int, object] = {}
+            held: Dict[int, List[object]] = {}
             for rid, rc in self._requests.items():
                 for p in rc.tables[gi]:
                     if p < 0:
                         continue
-                    if p in held:
+                    owners = g.pool.owners_of(p)
+                    if rid not in owners:
+                        raise CacheError(f"group {gi}: page {p} in {rid!r}'s table but owned by {owners!r}")
+                    if rid in held.setdefault(p, []) or len(held[p]) == len(owners):
                         raise CacheError(f"group {gi}: page {p} held by {held[p]!r} and {rid!r}")
-                    held[p] = rid
-                    if g.pool.owner_of(p) != rid:
-                        raise CacheError(f"group {gi}: page {p} in {rid!r}'s table but owned by {g.pool.owner_of(p)!r}")
+                    held[p].append(rid)
+            for p, rids in held.items():
+                if len(rids) != len(g.pool.owners_of(p)):
+                    raise CacheError(f"group {gi}: page {p} owned by {g.pool.owners_of(p)!r}, in the tables of {rids!r}")
             free = list(g.pool._free)
             if len(set(free)) != len(free):
                 raise CacheError(f"group {gi}: a page is on the free list twice")

@@ -78,6 +78,32 @@ class CacheStorage:
         for t in self.state:
             t[:, slot].zero_()
 
+    def copy_pages(self) -> None:
+        """Copies, in all layers, the shared pages that requests are about to write (`CacheManager.take_copies`), on the current stream."""
+        if not self.manager.has_copies:
+            return
+        from ..kernels import ops
+        for gi, pairs in enumerate(self.manager.take_copies()):
+            # a page that was copied and given back may have become another request's copy meanwhile: such pairs go in their order
+            while pairs:
+                sources, targets, n = set(), set(), 0
+                for s, d in pairs:
+                    if d in sources or d in targets or s in targets:
+                        break
+                    sources.add(s)
+                    targets.add(d)
+                    n += 1
+                own_values = not self.manager.paged_groups[gi].spec.values_in_keys
+                ops.copy_blocks([self.k_pages[gi]] + ([self.v_pages[gi]] if own_values else []), pairs[:n])
+                pairs = pairs[n:]
+
+    def copy_slot(self, source: int, target: int) -> None:
+        """The state of one request slot into another, in all layers."""
+        if self.state:
+            from ..kernels import ops
+            for i in range(0, len(self.state), 8):
+                ops.copy_blocks(self.state[i:i + 8], [(source, target)])
+
     def keys(self, cache_layer: int) -> torch.Tensor:
         kind, gi, li = self.manager.layer_location[cache_layer]
         assert kind == "paged"

@@ -22,6 +22,7 @@ class EngineOptions:
     cuda_graphs: bool = True            # replay captured decode steps
     step_graph_after: int = 2           # capture a general step's padded shape when it comes this many times (0: never)
     lookahead: bool = True              # launch the next decode step (its tokens taken on the device) before this one's are read
+    draft_tokens: int = 0               # most tokens that are drafted for a request and step, from its own text (0: none; at most 63)
     debug_poison: bool = False          # fill pages with NaN when they are given back: a read past a request's length shows
     device: str = "cuda:0"
 
@@ -35,6 +36,8 @@ class EngineOptions:
         for name in ("page_size", "ctx_size", "max_num_seqs", "max_num_batched_tokens", "prefill_chunk"):
             if getattr(self, name) <= 0:
                 raise ValueError(f"{name} must be positive, got {getattr(self, name)}")
+        if not 0 <= self.draft_tokens <= 63:
+            raise ValueError(f"draft_tokens must lie in 0..63, got {self.draft_tokens}")
         if self.max_tokens < 0:
             raise ValueError(f"max_tokens must not be negative, got {self.max_tokens}")
 

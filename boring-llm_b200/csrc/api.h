@@ -42,6 +42,11 @@ int bl_rope_kv_write(const float* qkv, const int* positions, const int* tok_req,
                      int max_pages, const float* inv_freq, int rot_half, float mscale,
                      void* q_out, void* k_cache, void* v_cache, int dtype,
                      int T, int H, int KV, int dh, int page_size, int pair_layout, void* stream);
+// ... into cache row cache_rows[t] of the token's request (null: row positions[t]); likewise the _rows forms further down.
+int bl_rope_kv_write_rows(const float* qkv, const int* positions, const int* cache_rows, const int* tok_req, const int* block_table,
+                          int max_pages, const float* inv_freq, int rot_half, float mscale,
+                          void* q_out, void* k_cache, void* v_cache, int dtype,
+                          int T, int H, int KV, int dh, int page_size, int pair_layout, void* stream);
 
 // Plain paged causal attention: one warp per (token, head), keys visited in ascending position.
 // Token t of request r = tok_req[t] stands at position ctx_len[r] - (cu_q[r+1] - cu_q[r]) + (t - cu_q[r])
@@ -174,6 +179,15 @@ int bl_qkv_rope_normed(const void* normed, const void* w_qkv, const void* bias, 
                        const int* tok_req, const int* block_table, int max_pages, const float* inv_freq, float mscale,
                        void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh, int page_size,
                        int pair_layout, void* stream);
+int bl_norm_qkv_rope_rows(const float* x, const void* norm_w, int norm_w_dtype, float eps, const void* w_qkv,
+                          const void* bias, int bias_dtype, const int* positions, const int* cache_rows, const int* tok_req,
+                          const int* block_table, int max_pages, const float* inv_freq, float mscale,
+                          void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
+                          int page_size, int pair_layout, void* stream);
+int bl_qkv_rope_normed_rows(const void* normed, const void* w_qkv, const void* bias, int bias_dtype, const int* positions,
+                            const int* cache_rows, const int* tok_req, const int* block_table, int max_pages, const float* inv_freq,
+                            float mscale, void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
+                            int page_size, int pair_layout, void* stream);
 // Programmatic dependent launch for the small kernels of a step (on by default): 0 launches them the ordinary way.
 void bl_set_dependent_launch(int on);
 

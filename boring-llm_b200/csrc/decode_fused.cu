@@ -29,7 +29,7 @@ struct FusedParams {
     void* out;                        // PLAIN: float [M, N]; SWIGLU: bfloat16 [M, N]; QKV: bfloat16 q [M, H * dh]
     int M, N, K, m_groups;
     // QKV only
-    const int* positions; const int* tok_req; const int* block_table; int max_pages;
+    const int* positions; const int* cache_rows; const int* tok_req; const int* block_table; int max_pages;     // cache_rows null: the positions
     const float* inv_freq; float mscale;
     __nv_bfloat16* k_cache; __nv_bfloat16* v_cache; int H, KV, dh, page_size, pair_layout;
 };
@@ -128,20 +128,21 @@ fused_norm_gemm_kernel(const FusedParams p) {
     if (!PRE)
         for (int k = threadIdx.x; k < K; k += WARPS * 32) nws[k] = bl_load_any(p.norm_w, p.norm_w_dtype, k);
     float e_b0 = 0.f, e_b1 = 0.f, e_cs = 1.f, e_sn = 0.f;
-    int e_pos = 0, e_page = -1;
+    int e_row = 0, e_page = -1;                       // the token's cache row and its page
     if (MODE == MODE_QKV && threadIdx.x < 8 * TOK) {
         const int c = threadIdx.x % 8, m = m0 + threadIdx.x / 8;
         if (m < p.M) {
             const bool inter = p.pair_layout == BL_PAIRS_INTERLEAVED;
             const int row_lo = hh * p.dh + (inter ? 2 * (jt * 8 + c) : jt * 8 + c), row_hi = inter ? row_lo + 1 : row_lo + p.dh / 2;
             if (p.bias) { e_b0 = bl_load_any(p.bias, p.bias_dtype, row_lo); e_b1 = bl_load_any(p.bias, p.bias_dtype, row_hi); }
-            e_pos = p.positions[m];
+            const int pos = p.positions[m];
+            e_row = p.cache_rows != nullptr ? p.cache_rows[m] : pos;
             if (hh < p.H + p.KV) {
-                const float angle = (float)e_pos * p.inv_freq[jt * 8 + c];
+                const float angle = (float)pos * p.inv_freq[jt * 8 + c];
                 e_cs = cosf(angle) * p.mscale; e_sn = sinf(angle) * p.mscale;
             }
             if (hh >= p.H && p.k_cache != nullptr)
-                e_page = p.block_table[(size_t)p.tok_req[m] * p.max_pages + e_pos / p.page_size];
+                e_page = p.block_table[(size_t)p.tok_req[m] * p.max_pages + e_row / p.page_size];
         }
     }
     if (PRE) fetch_pre_w(a2_lo, a2_hi, warp * 32 + UNROLL * WARPS * 32);
@@ -324,7 +325,7 @@ fused_norm_gemm_kernel(const FusedParams p) {
                     const bool is_k = hh < p.H + p.KV;
                     const int kvh = is_k ? hh - p.H : hh - p.H - p.KV;
                     __nv_bfloat16* dst = (is_k ? p.k_cache : p.v_cache) +
-                        (((size_t)e_page * p.KV + kvh) * p.page_size + e_pos % p.page_size) * p.dh;
+                        (((size_t)e_page * p.KV + kvh) * p.page_size + e_row % p.page_size) * p.dh;
                     dst[d0] = __float2bfloat16_rn(y0); dst[d1] = __float2bfloat16_rn(y1);
                 }
             }
@@ -428,7 +429,7 @@ extern "C" int bl_norm_gemm(const float* x, const int* row_idx, const void* norm
 namespace {
 
 int qkv_rope(const void* normed, const float* x, const void* norm_w, int norm_w_dtype, float eps, const void* w_qkv,
-             const void* bias, int bias_dtype, const int* positions, const int* tok_req, const int* block_table, int max_pages,
+             const void* bias, int bias_dtype, const int* positions, const int* cache_rows, const int* tok_req, const int* block_table, int max_pages,
              const float* inv_freq, float mscale, void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
              int page_size, int pair_layout, void* stream) {
     if (M <= 0) return 0;
@@ -444,7 +445,7 @@ int qkv_rope(const void* normed, const float* x, const void* norm_w, int norm_w_
     p.normed = (const __nv_bfloat16*)normed;
     p.x = x; p.norm_w = norm_w; p.norm_w_dtype = norm_w_dtype; p.eps = eps; p.w = (const __nv_bfloat16*)w_qkv;
     p.bias = bias; p.bias_dtype = bias_dtype; p.out = q_out; p.M = M; p.N = (H + 2 * KV) * dh; p.K = K;
-    p.positions = positions; p.tok_req = tok_req; p.block_table = block_table; p.max_pages = max_pages;
+    p.positions = positions; p.cache_rows = cache_rows; p.tok_req = tok_req; p.block_table = block_table; p.max_pages = max_pages;
     p.inv_freq = inv_freq; p.mscale = mscale; p.k_cache = (__nv_bfloat16*)k_cache; p.v_cache = (__nv_bfloat16*)v_cache;
     p.H = H; p.KV = KV; p.dh = dh; p.page_size = page_size; p.pair_layout = pair_layout;
     const int heads = k_cache ? H + 2 * KV : H;
@@ -460,7 +461,17 @@ extern "C" int bl_norm_qkv_rope(const float* x, const void* norm_w, int norm_w_d
                                 const int* block_table, int max_pages, const float* inv_freq, float mscale,
                                 void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
                                 int page_size, int pair_layout, void* stream) {
-    return qkv_rope(nullptr, x, norm_w, norm_w_dtype, eps, w_qkv, bias, bias_dtype, positions, tok_req, block_table, max_pages,
+    return bl_norm_qkv_rope_rows(x, norm_w, norm_w_dtype, eps, w_qkv, bias, bias_dtype, positions, nullptr, tok_req, block_table, max_pages,
+                                 inv_freq, mscale, q_out, k_cache, v_cache, M, K, H, KV, dh, page_size, pair_layout, stream);
+}
+
+// ... into cache row cache_rows[m] of the token's request instead of row positions[m] (null: the positions).
+extern "C" int bl_norm_qkv_rope_rows(const float* x, const void* norm_w, int norm_w_dtype, float eps, const void* w_qkv,
+                                     const void* bias, int bias_dtype, const int* positions, const int* cache_rows, const int* tok_req,
+                                     const int* block_table, int max_pages, const float* inv_freq, float mscale,
+                                     void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
+                                     int page_size, int pair_layout, void* stream) {
+    return qkv_rope(nullptr, x, norm_w, norm_w_dtype, eps, w_qkv, bias, bias_dtype, positions, cache_rows, tok_req, block_table, max_pages,
                     inv_freq, mscale, q_out, k_cache, v_cache, M, K, H, KV, dh, page_size, pair_layout, stream);
 }
 
@@ -469,7 +480,15 @@ extern "C" int bl_qkv_rope_normed(const void* normed, const void* w_qkv, const v
                                   const int* tok_req, const int* block_table, int max_pages, const float* inv_freq, float mscale,
                                   void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
                                   int page_size, int pair_layout, void* stream) {
+    return bl_qkv_rope_normed_rows(normed, w_qkv, bias, bias_dtype, positions, nullptr, tok_req, block_table, max_pages, inv_freq, mscale, q_out,
+                                   k_cache, v_cache, M, K, H, KV, dh, page_size, pair_layout, stream);
+}
+
+extern "C" int bl_qkv_rope_normed_rows(const void* normed, const void* w_qkv, const void* bias, int bias_dtype, const int* positions,
+                                       const int* cache_rows, const int* tok_req, const int* block_table, int max_pages, const float* inv_freq,
+                                       float mscale, void* q_out, void* k_cache, void* v_cache, int M, int K, int H, int KV, int dh,
+                                       int page_size, int pair_layout, void* stream) {
     if (M > 0 && normed == nullptr) BL_FAIL("bl_qkv_rope_normed: no rows");
-    return qkv_rope(normed, nullptr, nullptr, BL_F32, 0.f, w_qkv, bias, bias_dtype, positions, tok_req, block_table, max_pages,
+    return qkv_rope(normed, nullptr, nullptr, BL_F32, 0.f, w_qkv, bias, bias_dtype, positions, cache_rows, tok_req, block_table, max_pages,
                     inv_freq, mscale, q_out, k_cache, v_cache, M, K, H, KV, dh, page_size, pair_layout, stream);
 }

@@ -218,6 +218,7 @@ __device__ __forceinline__ void bl_store4(__nv_bfloat16* p, float a, float b, fl
 // aligned: a work item is four neighbouring pairs of a head, read and written with one vector access each.
 template <typename TT, bool VEC>
 __global__ void rope_kv_write_kernel(const float* qkv /* written by the kernel before */, const int* __restrict__ positions,
+                                     const int* __restrict__ cache_rows /* null: the positions */,
                                      const int* __restrict__ tok_req, const int* __restrict__ block_table,
                                      int max_pages, const float* __restrict__ inv_freq, int rot_half,
                                      float mscale, TT* __restrict__ q_out, TT* __restrict__ k_cache,
@@ -232,9 +233,10 @@ __global__ void rope_kv_write_kernel(const float* qkv /* written by the kernel b
     size_t page_base = 0;
     bool write = k_cache != nullptr;
     if (write) {
-        const int page = block_table[(size_t)tok_req[t] * max_pages + pos / page_size];
+        const int at = cache_rows != nullptr ? cache_rows[t] : pos;
+        const int page = block_table[(size_t)tok_req[t] * max_pages + at / page_size];
         if (page < 0) write = false;       // the host never schedules this; keep memory safe anyway
-        page_base = ((size_t)(page < 0 ? 0 : page) * KV) * page_size * dh + (size_t)(pos % page_size) * dh;
+        page_base = ((size_t)(page < 0 ? 0 : page) * KV) * page_size * dh + (size_t)(at % page_size) * dh;
     }
     // the rotation of pair j is the same for every head of the token: worked out once, into shared memory
     extern __shared__ __align__(16) float cs_sn[];                     // [rot_half] cos, then [rot_half] sin
@@ -305,6 +307,15 @@ extern "C" int bl_rope_kv_write(const float* qkv, const int* positions, const in
                                 const int* block_table, int max_pages, const float* inv_freq,
                                 int rot_half, float mscale, void* q_out, void* k_cache, void* v_cache,
                                 int dtype, int T, int H, int KV, int dh, int page_size, int pair_layout, void* stream) {
+    return bl_rope_kv_write_rows(qkv, positions, nullptr, tok_req, block_table, max_pages, inv_freq, rot_half, mscale, q_out, k_cache,
+                                 v_cache, dtype, T, H, KV, dh, page_size, pair_layout, stream);
+}
+
+// ... into cache row cache_rows[t] of the token's request instead of row positions[t] (drafted tokens: several may share a position).
+extern "C" int bl_rope_kv_write_rows(const float* qkv, const int* positions, const int* cache_rows, const int* tok_req,
+                                     const int* block_table, int max_pages, const float* inv_freq,
+                                     int rot_half, float mscale, void* q_out, void* k_cache, void* v_cache,
+                                     int dtype, int T, int H, int KV, int dh, int page_size, int pair_layout, void* stream) {
     if (T <= 0) return 0;
     if (pair_layout != BL_PAIRS_HALVES && pair_layout != BL_PAIRS_INTERLEAVED)
         BL_FAIL("bl_rope_kv_write: unknown pair layout %d (0: (j, j + n_rot/2), 1: (2j, 2j + 1))", pair_layout);
@@ -317,7 +328,7 @@ extern "C" int bl_rope_kv_write(const float* qkv, const int* positions, const in
     const bool vec = pair_layout == BL_PAIRS_HALVES && rot_half * 2 == dh && rot_half % 4 == 0 && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)inv_freq & 3) == 0 &&
                      ((uintptr_t)q_out % (4 * elem)) == 0 && ((uintptr_t)k_cache % (4 * elem)) == 0 && ((uintptr_t)v_cache % (4 * elem)) == 0;
     const size_t smem = (size_t)rot_half * 8;
-#define BL_ROPE(TT, VEC) BL_CUDA(bl_launch_dependent(rope_kv_write_kernel<TT, VEC>, dim3(T), dim3(128), smem, s, qkv, positions, tok_req, \
+#define BL_ROPE(TT, VEC) BL_CUDA(bl_launch_dependent(rope_kv_write_kernel<TT, VEC>, dim3(T), dim3(128), smem, s, qkv, positions, cache_rows, tok_req, \
         block_table, max_pages, inv_freq, rot_half, mscale, (TT*)q_out, (TT*)k_cache, (TT*)v_cache, H, KV, dh, page_size, pair_layout))
     if (dtype == BL_F32) { if (vec) BL_ROPE(float, true); else BL_ROPE(float, false); }
     else if (dtype == BL_BF16) { if (vec) BL_ROPE(__nv_bfloat16, true); else BL_ROPE(__nv_bfloat16, false); }

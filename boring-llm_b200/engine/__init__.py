@@ -1,7 +1,7 @@
-from .runner import ModelRunner, StepEntry, OutOfPages, StepError
+from .runner import ModelRunner, StepEntry, TreeEntry, OutOfPages, StepError
 from .scheduler import Scheduler, Request, ScheduledStep, AdmissionError
 from .engine import Engine, generate
 from ..sampling.params import SamplingParams
 
-__all__ = ["ModelRunner", "StepEntry", "OutOfPages", "StepError", "Scheduler", "Request", "ScheduledStep",
+__all__ = ["ModelRunner", "StepEntry", "TreeEntry", "OutOfPages", "StepError", "Scheduler", "Request", "ScheduledStep",
            "AdmissionError", "Engine", "generate", "SamplingParams"]

@@ -6,18 +6,20 @@ scheduler builds each step's batch, the runner computes logits, the device sampl
 """
 from __future__ import annotations
 
+import copy
 import itertools
 import time
 from typing import Dict, List, Optional, Sequence
 
 import torch
 
+from ..cache import CacheError
 from ..config import EngineOptions
 from ..models.loading import load_model, load_random_model
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
-from .runner import ModelRunner, StepEntry
-from .scheduler import RUNNING, Request, Scheduler
+from .runner import ModelRunner, OutOfPages, StepEntry, TreeEntry
+from .scheduler import RUNNING, WAITING, Request, Scheduler
 
 
 class Engine:
@@ -41,6 +43,9 @@ class Engine:
         self.runner = ModelRunner(self.model, options)
         self.scheduler = Scheduler(self.runner.cache, options)
         self.sampler = Sampler(options.device)
+        if options.draft_tokens and not self.runner.takes_trees:
+            raise ValueError("draft_tokens: this model's mixers keep state of their own beside pages, or attend in a way of their own; "
+                             "drafted tokens could not be taken back")
         self._ids = itertools.count()
         self._inflight = None                 # (scheduled step, PendingDecode): launched, tokens not read yet
         self.stats_time = {"engine_steps": 0, "step_seconds": 0.0}
@@ -85,6 +90,15 @@ class Engine:
                 return []
             # the third item is the request itself: its token history is only put together if a penalty asks for it
             rows = [(r.params, r.rng, r) for r, s in zip(sched.requests, sched.samples) if s]
+            if self.options.draft_tokens:
+                said = self._drafted_step(sched, rows)
+                if said is None:
+                    sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
+                    return self._finish_step(sched, sampled, t0)
+                self.runner.check_kernels()
+                self.stats_time["engine_steps"] += 1
+                self.stats_time["step_seconds"] += time.perf_counter() - t0
+                return self.scheduler.apply_drafted(sched, said)
             pending = self.runner.launch_decode(sched.entries, rows) if self.options.lookahead else None
             if pending is None:
                 sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
@@ -113,6 +127,34 @@ class Engine:
             nxt = None                            # every row of the step ahead has ended: nobody reads it
         self._inflight = nxt
         return done
+
+    def _drafted_step(self, sched, rows):
+        """A step that only decodes, with drafted tokens; None when it is another kind of step, nothing is drafted, or the cache has
+        no pages for the drafts (then nothing has been done)."""
+        trees = self.scheduler.draft(sched)
+        if trees is None:
+            return None
+        try:
+            return self.runner.step_tree([TreeEntry(e.request_id, *tree) for e, tree in zip(sched.entries, trees)], rows)
+        except OutOfPages:
+            return None
+
+    def fork(self, request, params: Optional[SamplingParams] = None, request_id=None) -> Request:
+        """A second running request that goes on from where `request` (a `Request` that runs, its prompt computed) is, with parameters
+        and a generator of its own. The pages of what both have in common are shared."""
+        self.drain()
+        if request.state != RUNNING or request.remaining != 1:
+            raise ValueError(f"request {request.request_id!r} cannot be forked: it has ended, or its prompt is not computed yet")
+        return self._fork(request, params if params is not None else copy.copy(request.params), request_id, request.num_computed,
+                          len(request.output))
+
+    def _fork(self, request, params, request_id, n_keep: int, n_output: int) -> Request:
+        if not params.eos_token_ids and not params.ignore_eos:
+            params.eos_token_ids = tuple(getattr(self.config, "eos_token_ids", ()))
+        source = self.runner.cache.get(request.request_id)
+        new = self.scheduler.fork(request, request_id if request_id is not None else next(self._ids), params, n_keep, n_output)
+        self.runner.storage.copy_slot(source.slot, self.runner.cache.get(new.request_id).slot)
+        return new
 
     def _abort_rows(self, requests) -> None:
         seen = set()
@@ -147,23 +189,51 @@ class Engine:
     def generate(self, prompts: Sequence[Sequence[int]], n_predict: int = 40, temperature: float = 0.0,
                  seed: int = 0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
                  repeat_penalty: float = 1.0, repeat_last_n: int = 64,
-                 eos_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False) -> List[List[int]]:
+                 eos_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False, n: int = 1) -> List[List[int]]:
         """Generated token ids for each prompt (lists of token ids), in the prompts' order. Request i
         draws from a generator seeded with `seed + i`, so a batch and the same prompts one by one
-        give the same tokens."""
-        reqs = []
+        give the same tokens. `n` > 1: as many answers to each prompt, one behind the other (answer k of prompt i is request
+        i * n + k); where the model keeps nothing but pages a prompt is computed once and its answers share its pages."""
+        if n < 1:
+            raise ValueError(f"n must be positive, got {n}")
+        reqs, waiting = [], []
         for i, prompt in enumerate(prompts):
-            params = SamplingParams(n_predict=n_predict, temperature=temperature, seed=seed + i, top_k=top_k,
-                                    top_p=top_p, min_p=min_p, repeat_penalty=repeat_penalty,
-                                    repeat_last_n=repeat_last_n,
-                                    eos_token_ids=tuple(eos_token_ids) if eos_token_ids is not None else (),
-                                    ignore_eos=ignore_eos)
-            reqs.append(self.add_request(prompt, params))
+            answers = []
+            for k in range(n):
+                params = SamplingParams(n_predict=n_predict, temperature=temperature, seed=seed + i * n + k, top_k=top_k,
+                                        top_p=top_p, min_p=min_p, repeat_penalty=repeat_penalty,
+                                        repeat_last_n=repeat_last_n,
+                                        eos_token_ids=tuple(eos_token_ids) if eos_token_ids is not None else (),
+                                        ignore_eos=ignore_eos)
+                if k and len(prompt) > 1 and not self.runner.cache.state_groups:
+                    waiting.append((answers[0], prompt, params, i * n + k))
+                    answers.append(None)
+                else:
+                    answers.append(self.add_request(prompt, params))
+            reqs += answers
+        while waiting:
+            # a source whose prompt is computed is forked in front of the prompt's last token, which each answer runs itself: its logits
+            # are what the first tokens are drawn from. One that has ended or waits again by then, or for want of a slot: another request.
+            left = []
+            for source, prompt, params, at in waiting:
+                if source.state == WAITING and not source.output or source.state == RUNNING and source.num_computed < len(prompt):
+                    left.append((source, prompt, params, at))
+                elif source.state == RUNNING and self.runner.cache.has_free_slot() and params.n_predict != 0:
+                    try:
+                        reqs[at] = self._fork(source, params, None, len(prompt) - 1, 0)
+                    except CacheError:                # a window has passed the prompt's end: its pages are gone
+                        reqs[at] = self.add_request(prompt, params)
+                else:
+                    reqs[at] = self.add_request(prompt, params)
+            waiting = left
+            if waiting:
+                self.step()
         self.run_until_done()
         return [list(r.output) for r in reqs]
 
     def stats(self) -> dict:
         s = dict(self.runner.cache.stats())
+        s.update(drafted_tokens=self.runner.drafted, accepted_tokens=self.runner.accepted)
         s.update(steps=self.runner.steps, tokens_run=self.runner.tokens_run,
                  preemptions=self.scheduler.num_preemptions, **self.stats_time)
         return s

@@ -11,6 +11,7 @@ scheduler's (or the trace's) business.
 from __future__ import annotations
 
 import array
+import copy
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
@@ -21,6 +22,7 @@ from ..cache import CacheManager, CacheStorage
 from ..config import EngineOptions
 from ..models.loading import torch_dtype
 from ..parts import StepContext, StepPlan
+from .draft import MAX_NODES, tree_masks
 
 
 @dataclass
@@ -29,6 +31,15 @@ class StepEntry:
     request_id: object
     tokens: Sequence[int]
     want: Sequence[int] = ()
+
+
+@dataclass
+class TreeEntry:
+    """The nodes of a tree of drafted tokens of one live request. Node 0 is a certain token (the one to feed next, `parents[0]` -1),
+    node i > 0 a guess at what follows node `parents[i]` < i."""
+    request_id: object
+    tokens: Sequence[int]
+    parents: Sequence[int]
 
 
 class OutOfPages(RuntimeError):
@@ -41,6 +52,7 @@ class StepError(ValueError):
 
 GRAPH_MAX_BATCH = 64          # decode steps of up to this many requests replay a captured CUDA graph
 STEP_GRAPH_MAX_WANTED = 64    # general steps that want more rows of logits than this are launched kernel by kernel
+TREE_GRAPH_MAX_NODES = 512    # steps of drafted trees with up to this many nodes replay a captured graph
 STEP_GRAPH_CACHE = 48         # captured general steps kept (least recently used goes first)
 
 
@@ -146,6 +158,114 @@ class _StepGraph:
         with torch.cuda.graph(self.graph, pool=runner._step_graph_pool()):
             self.logits = runner.model.forward(self.ctx)
         self.kernels = ops.launch_count - before
+
+
+class _TreeBatch:
+    """The buffers of a step of drafted trees for T nodes of R requests, and the step itself: forward pass, a token sampled behind every
+    node, acceptance and the moves of the accepted rows in the caches of all groups. May be captured and replayed."""
+
+    def __init__(self, runner: "ModelRunner", T: int, R: int):
+        G, W = len(runner.cache.paged_groups), runner._table_width
+        sizes = [("mask", 2 * T), ("token_ids", T), ("positions", T), ("cache_rows", T), ("tok_req", T), ("cu_q", R + 1), ("ctx_len", R),
+                 ("slots", R), ("logit_rows", T), ("tables", G * R * W), ("temperature", T), ("top_k", T), ("top_p", T), ("min_p", T),
+                 ("uniform", T)]
+        total = sum(n for _, n in sizes)
+        self.T, self.R = T, R
+        self.host = torch.zeros(total, dtype=torch.int32).pin_memory()
+        self.dev = torch.zeros(total, dtype=torch.int32, device=runner.device)
+        host, o = self.host.numpy(), 0
+        self.h: Dict[str, np.ndarray] = {}
+        self.d: Dict[str, torch.Tensor] = {}
+        for name, n in sizes:
+            self.h[name], self.d[name] = host[o:o + n], self.dev[o:o + n]
+            o += n
+        self.h["mask"] = self.h["mask"].view(np.uint64)          # the first field: aligned to eight bytes
+        self.d["mask"] = self.d["mask"].view(torch.int64)
+        self.h["tables"] = self.h["tables"].reshape(G, R, W)
+        for name in ("temperature", "top_p", "min_p", "uniform"):
+            self.h[name], self.d[name] = self.h[name].view(np.float32), self.d[name].view(torch.float32)
+        self.h["logit_rows"][:] = np.arange(T, dtype=np.int32)
+        d = self.d
+        self.ctx = StepContext(
+            dtype=runner.dtype, device=runner.device, T=T, R=R, token_ids=d["token_ids"], positions=d["positions"], tok_req=d["tok_req"],
+            cu_q=d["cu_q"], ctx_len=d["ctx_len"], slots=d["slots"], logit_rows=d["logit_rows"],
+            block_tables=[d["tables"][g * R * W:(g + 1) * R * W].view(R, W) for g in range(G)], q_lens=[], ctx_lens=[], slot_list=[],
+            storage=runner.storage, fast=runner.fast, tree_mask=d["mask"], cache_rows=d["cache_rows"])
+        self.found_host = None
+        self.graph = None
+        self.uses = 0
+        self.kernels = 0
+
+    def fill(self, runner: "ModelRunner", entries, rows, masks) -> list:
+        """The step's numbers into the host buffer. Returns, per entry that draws, its generator's state after each depth's number: all
+        nodes of a depth get the number that the token at their place would be drawn with."""
+        h, t0, draws = self.h, 0, []
+        n_all = sum(len(e.tokens) for e in entries)
+        h["tables"][...] = -1
+        for r, (e, (params, rng, _), mask) in enumerate(zip(entries, rows, masks)):
+            rc, n = runner.cache.get(e.request_id), len(e.tokens)
+            at = slice(t0, t0 + n)
+            depth = np.fromiter((m.bit_count() - 1 for m in mask), dtype=np.int32, count=n)
+            h["mask"][at] = np.array(mask, dtype=np.uint64)
+            h["token_ids"][at] = np.asarray(e.tokens, dtype=np.int32)
+            h["positions"][at] = rc.num_tokens + depth
+            h["cache_rows"][at] = np.arange(rc.num_tokens, rc.num_tokens + n, dtype=np.int32)
+            h["tok_req"][at] = r
+            h["cu_q"][r], h["ctx_len"][r], h["slots"][r] = t0, rc.num_tokens + n, rc.slot
+            for gi, tab in enumerate(rc.tables):
+                h["tables"][gi, r, :len(tab)] = tab
+            h["temperature"][at], h["top_k"][at], h["top_p"][at], h["min_p"][at] = params.temperature, params.top_k, params.top_p, params.min_p
+            states = []
+            if params.temperature > 0:
+                ahead, numbers = copy.copy(rng), []
+                for _ in range(int(depth.max()) + 1):
+                    numbers.append(ahead.next_f32())
+                    states.append(ahead.state)
+                h["uniform"][at] = np.asarray(numbers, dtype=np.float32)[depth]
+            draws.append(states)
+            t0 += n
+        R, pads = len(entries), self.T - n_all
+        h["mask"][t0:] = 1
+        for name in ("token_ids", "positions", "cache_rows", "top_k"):
+            h[name][t0:] = 0
+        h["temperature"][t0:] = 0.0
+        h["tok_req"][t0:] = np.arange(R, R + pads, dtype=np.int32)
+        h["cu_q"][R:R + pads + 1] = np.arange(t0, self.T + 1, dtype=np.int32)
+        h["cu_q"][R + pads + 1:] = self.T
+        h["ctx_len"][R:] = 1
+        h["slots"][R:] = runner.storage.trash_slot
+        h["tables"][:, R:, 0] = runner.storage.trash_page
+        return draws
+
+    def run(self, runner: "ModelRunner") -> None:
+        from ..kernels import ops
+        d = self.d
+        logits = runner.model.forward(self.ctx)
+        sampled = torch.empty(self.T, dtype=torch.int32, device=runner.device)
+        ops.sample(logits, d["temperature"], d["top_k"], d["top_p"], d["min_p"], d["uniform"], sampled)
+        for k, v, table in zip(runner.storage.k_pages, runner.storage.v_pages, self.ctx.block_tables):
+            self.counts, _, self.tokens = ops.accept_tree(sampled, d["token_ids"], d["mask"], d["cu_q"], d["ctx_len"], k, v, table)
+
+    def capture(self, runner: "ModelRunner") -> None:
+        from ..kernels import ops
+        torch.cuda.synchronize()
+        before = ops.launch_count
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, pool=runner._step_graph_pool()):
+            self.run(runner)
+        self.kernels = ops.launch_count - before
+
+    def read(self, R: int):
+        """(counts [R], tokens [R, 64]) on the host, once the step has run."""
+        if self.found_host is None:
+            self.found_host = (torch.empty(self.R, dtype=torch.int32).pin_memory(), torch.empty((self.R, MAX_NODES), dtype=torch.int32).pin_memory())
+        counts, tokens = self.found_host
+        counts.copy_(self.counts, non_blocking=True)
+        tokens.copy_(self.tokens, non_blocking=True)
+        done = torch.cuda.Event()
+        done.record()
+        done.synchronize()
+        return counts.numpy()[:R], tokens.numpy()[:R]
 
 
 class PendingDecode:
@@ -287,6 +407,9 @@ class ModelRunner:
         self._step_shapes_seen: Dict[tuple, int] = {}
         self._graph_pool = None
         self._graph_safe: Optional[bool] = None
+        self._tree_graphs: Dict[tuple, "_TreeBatch"] = {}    # padded (nodes, requests) -> captured step of drafted trees
+        self._takes_trees: Optional[bool] = None
+        self.drafted = self.accepted = 0               # drafted tokens run and those of them that were accepted
         self._waits_unchecked = False                  # a step ran kernels with bounded waits since the last check
         self._table_width = -(-(-(-options.ctx_size // options.page_size)) // 8) * 8
 
@@ -308,6 +431,13 @@ class ModelRunner:
         if self.cache.state_groups:
             raise StepError(f"request {request_id!r}: state of fixed size cannot be truncated; recompute from the start")
         self.cache.truncate(request_id, n_keep)
+
+    def fork_request(self, request_id, new_id, n_keep: Optional[int] = None) -> None:
+        """A new request that holds the first `n_keep` tokens (default: all) of a live one. Pages are shared until one of the two writes
+        to them; state of fixed size is copied (then `n_keep` must be all)."""
+        source = self.cache.get(request_id)
+        new = self.cache.fork(request_id, new_id, n_keep)
+        self.storage.copy_slot(source.slot, new.slot)
 
     # ---- the step ----------------------------------------------------------------------------------
     def _host_buffer(self, n_ints: int) -> torch.Tensor:
@@ -334,6 +464,7 @@ class ModelRunner:
         is returned instead, for `collect_decode`. With `from_device` the rows' tokens are the ones the
         replay before this one sampled (same requests in the same rows): they are taken on the device,
         so the step can be launched before the host has seen them."""
+        self.storage.copy_pages()
         R = len(entries)
         rows = 1
         while rows < R:
@@ -503,9 +634,9 @@ class ModelRunner:
             n_have = held.num_tokens if held else 0
             if n_have + len(e.tokens) > self.options.ctx_size:
                 raise StepError(f"request {e.request_id!r}: {n_have + len(e.tokens)} tokens exceed the context size {self.options.ctx_size}")
-            total = -(-(n_have + len(e.tokens)) // page)
+            each = self.cache.pages_needed(e.request_id, len(e.tokens)) if held else [-(-len(e.tokens) // page)] * len(need)
             for gi in range(len(need)):
-                need[gi] += max(0, total - (len(held.tables[gi]) if held else 0))
+                need[gi] += each[gi]
         free = self.cache.free_pages()
         if any(n > f for n, f in zip(need, free)):
             raise OutOfPages(f"the step needs {need} pages per group, {free} are free")
@@ -535,7 +666,7 @@ class ModelRunner:
             room = rc.num_tokens < page * len(rc.tables[0]) if rc.tables else True
             for tab in rc.tables[1:]:
                 room = room and rc.num_tokens < page * len(tab)
-            if not room:
+            if not room or rc.forked and any(self.cache.pages_needed(e.request_id, 1)):
                 return False
             seen.add(e.request_id)
         return len(seen) == len(entries)
@@ -545,6 +676,7 @@ class ModelRunner:
         in one pinned copy. A batch whose padded shape has been seen before replays a captured graph (`_StepGraph`);
         otherwise the kernels are launched one by one."""
         self.last_step_graph_kernels = 0
+        self.storage.copy_pages()
         R = len(entries)
         T = sum(len(e.tokens) for e in entries)
         N = sum(len(e.want) for e in entries)
@@ -676,6 +808,97 @@ class ModelRunner:
         self.last_step_graph_kernels = gr.kernels
         self.graph_steps += 1
         return gr.logits[:N]
+
+    # ---- steps of drafted trees --------------------------------------------------------------------------
+    @property
+    def takes_trees(self) -> bool:
+        """Whether this model runs steps of drafted trees (`step_tree`)."""
+        if self._takes_trees is None:
+            self._takes_trees = bool(getattr(self.model, "takes_trees", False))
+        return self._takes_trees
+
+    def step_tree(self, entries: Sequence[TreeEntry], rows) -> List[List[int]]:
+        """Runs a tree of drafted tokens for each entry's request, samples a token behind every node, and keeps of each tree the longest path
+        from node 0 whose tokens are the sampled ones. Returns, per entry, the tokens sampled along that path (one more than
+        there were drafted tokens on it): the same that one step after the other would have sampled, from the same random numbers.
+        All but the last are in the cache then, behind the token of node 0. `rows` holds one (params, generator, history)
+        per entry; a repeat penalty is refused (StepError), as is a model that keeps more of a request than pages."""
+        if not self.takes_trees:
+            raise StepError("this model does not run trees of drafted tokens: a mixer keeps state, or attends in a way of its own")
+        if not entries or len(rows) != len(entries):
+            raise StepError("a step of drafted trees needs an entry, and (params, generator, history) for each")
+        seen, masks = set(), []
+        for e, (params, _, _) in zip(entries, rows):
+            if e.request_id in seen:
+                raise StepError(f"request {e.request_id!r} appears twice in one step")
+            seen.add(e.request_id)
+            if len(e.tokens) != len(e.parents) or not 0 < len(e.tokens) <= MAX_NODES:
+                raise StepError(f"request {e.request_id!r}: a tree has 1 to {MAX_NODES} nodes and a parent for each")
+            for t in e.tokens:
+                if not 0 <= int(t) < self.vocab_size:
+                    raise StepError(f"request {e.request_id!r}: token id {t} is outside the vocabulary (0..{self.vocab_size - 1})")
+            try:
+                masks.append(tree_masks(e.parents))
+            except ValueError as err:
+                raise StepError(f"request {e.request_id!r}: {err}") from None
+            if params.repeat_penalty != 1.0:
+                raise StepError(f"request {e.request_id!r}: a repeat penalty needs the tokens one after the other")
+            rc = self.cache.find(e.request_id)
+            if rc is None:
+                raise StepError(f"request {e.request_id!r} is not live")
+            if rc.num_tokens + len(e.tokens) > self.options.ctx_size:
+                raise StepError(f"request {e.request_id!r}: {rc.num_tokens + len(e.tokens)} tokens exceed the context size {self.options.ctx_size}")
+        need = [sum(n) for n in zip(*(self.cache.pages_needed(e.request_id, len(e.tokens)) for e in entries))]
+        free = self.cache.free_pages()
+        if any(n > f for n, f in zip(need, free)):
+            raise OutOfPages(f"the step needs {need} pages per group, {free} are free")
+        if self.options.debug_poison:
+            self.storage.poison_freed_pages()
+        for e in entries:
+            self.cache.reserve(e.request_id, len(e.tokens))
+        self.storage.copy_pages()
+        R, T = len(entries), sum(len(e.tokens) for e in entries)
+        shape = None
+        if self._graphs_usable(entries) and T <= TREE_GRAPH_MAX_NODES:
+            # padded to a shape that other steps share: each padding node a request of its own on the spare page, then empty requests
+            T_b = -(-T // 16) * 16 if T <= 64 else -(-T // 64) * 64
+            shape = (T_b, -(-(R + T_b - T) // 8) * 8)
+            batch = self._tree_graphs.pop(shape, None)
+            if batch is None and len(self._tree_graphs) >= STEP_GRAPH_CACHE:
+                del self._tree_graphs[next(iter(self._tree_graphs))]
+            batch = self._tree_graphs[shape] = batch if batch is not None else _TreeBatch(self, *shape)   # most recently used last
+            batch.uses += 1
+        else:
+            batch = _TreeBatch(self, T, R)
+        draws = batch.fill(self, entries, rows, masks)
+        batch.dev.copy_(batch.host, non_blocking=True)
+        self.last_h2d_bytes = 4 * batch.host.numel()
+        self.last_step_graph_kernels = 0
+        if batch.graph is not None:
+            batch.graph.replay()
+            self.last_step_graph_kernels = batch.kernels
+            self.graph_steps += 1
+        else:
+            batch.run(self)
+        self._waits_unchecked = self._waits_unchecked or self.fast
+        counts, tokens = batch.read(R)
+        self.last_d2h_bytes = 4 * R * (1 + MAX_NODES)
+        if shape is not None and batch.graph is None and 0 < self.options.step_graph_after <= batch.uses:
+            batch.capture(self)                          # (this step has run; the capture itself runs nothing)
+        said = []
+        for r, (e, (params, rng, _)) in enumerate(zip(entries, rows)):
+            n = int(counts[r])
+            if n < 1:
+                raise StepError(f"request {e.request_id!r}: the step accepted no node (node 0 is always accepted)")
+            self.cache.commit(e.request_id, n)
+            if params.temperature > 0:
+                rng.state = draws[r][n - 1]
+            said.append([int(t) for t in tokens[r, :n]])
+            self.drafted += len(e.tokens) - 1
+            self.accepted += n - 1
+        self.steps += 1
+        self.tokens_run += T
+        return said
 
     def check_kernels(self) -> None:
         """The tcgen05 kernels bound every wait on a barrier and record it when a bound runs out instead of

@@ -29,6 +29,7 @@ from typing import Deque, Dict, List, Optional, Sequence
 from ..cache import CacheManager
 from ..config import EngineOptions
 from ..sampling.params import SamplingParams, XorShift64
+from .draft import History
 from .runner import StepEntry
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
@@ -51,6 +52,7 @@ class Request:
     arrival: int = 0
     preemptions: int = 0
     rng: Optional[XorShift64] = None
+    history: Optional[History] = None     # of its tokens so far, once drafts have been asked for
 
     @property
     def tokens(self) -> List[int]:
@@ -223,6 +225,28 @@ class Scheduler:
         return ScheduledStep([StepEntry(req.request_id, [0], [0]) for req in prev.requests], list(prev.requests),
                              [True] * len(prev.requests))
 
+    def draft(self, step: ScheduledStep) -> Optional[List[tuple]]:
+        """(tokens, parents) of a tree of drafted tokens for every request of a step that only decodes, or None: it is another kind
+        of step, a request has a penalty on repeated tokens (its tokens would have to be sampled one after the other), or
+        nothing is drafted for any. The trees respect the token budget, the context and what each request may still say."""
+        if not step.entries or not all(s and len(e.tokens) == 1 for e, s in zip(step.entries, step.samples)):
+            return None
+        if any(r.params.repeat_penalty != 1.0 for r in step.requests):
+            return None
+        room = self.options.max_num_batched_tokens // len(step.requests)
+        trees, drafted = [], 0
+        for req in step.requests:
+            if req.history is None:
+                req.history = History()
+            req.history.extend(req.token_slice(len(req.history.tokens), len(req.prompt) + len(req.output)))
+            # node i goes to cache row num_computed + i; no drafted token may lie behind the last one that can be wanted
+            depth = min(self.options.draft_tokens, req.max_new - len(req.output) - 1)
+            nodes = min(self.options.draft_tokens + 1, room, self.options.ctx_size - req.num_computed)
+            tree = req.history.draft(max(nodes, 1), depth=max(depth, 0))
+            drafted += len(tree[0]) - 1
+            trees.append(tree)
+        return trees if drafted else None
+
     def apply(self, step: ScheduledStep, sampled: Sequence[int]) -> List[Request]:
         """Records a finished step: `sampled` holds one token for every entry with `samples` true, in
         order. Returns the requests that finished. An end-of-generation token is returned but not
@@ -235,23 +259,56 @@ class Scheduler:
                     next(it, None)                            # its row's token belongs to nobody
                 continue
             req.num_computed += len(e.tokens)
-            if not samp:
-                continue
-            tok = int(next(it))
-            req.output.append(tok)
-            p = req.params
-            if not p.ignore_eos and tok in p.eos_token_ids:
-                reason = "stop"
-            elif len(req.output) >= req.max_new:
-                reason = "length"
-            elif len(req.prompt) + len(req.output) >= self.options.ctx_size:
-                reason = "length"
-            else:
-                continue
-            self.running.remove(req)
-            self._finish(req, reason, live=True)
-            done.append(req)
+            if samp:
+                self._say(req, int(next(it)), done)
         return done
+
+    def apply_drafted(self, step: ScheduledStep, said: Sequence[Sequence[int]]) -> List[Request]:
+        """Records a finished step of drafted trees: `said[i]` are the tokens that entry i's request has said, each but the last of
+        which is in the cache (in front of them the one that the entry brought). Returns the requests that finished."""
+        done: List[Request] = []
+        for req, tokens in zip(step.requests, said):
+            if req.state != RUNNING:
+                continue
+            req.num_computed += len(tokens)
+            for tok in tokens:
+                self._say(req, int(tok), done)
+                if req.state != RUNNING:                      # what it would have said behind its end belongs to nobody
+                    break
+        return done
+
+    def _say(self, req: Request, tok: int, done: List[Request]) -> None:
+        req.output.append(tok)
+        p = req.params
+        if not p.ignore_eos and tok in p.eos_token_ids:
+            reason = "stop"
+        elif len(req.output) >= req.max_new:
+            reason = "length"
+        elif len(req.prompt) + len(req.output) >= self.options.ctx_size:
+            reason = "length"
+        else:
+            return
+        self.running.remove(req)
+        self._finish(req, reason, live=True)
+        done.append(req)
+
+    def fork(self, source: Request, request_id, params: SamplingParams, n_keep: int, n_output: int) -> Request:
+        """A running request that knows a running one's prompt and the first `n_output` tokens of its answer, with parameters and a
+        generator of its own. The first `n_keep` of these are in its cache, in pages that the two share until one of them writes
+        there; the others it computes itself."""
+        if source.state != RUNNING:
+            raise AdmissionError(f"request {source.request_id!r} is not running: it cannot be forked")
+        if not self.cache.has_free_slot():
+            raise AdmissionError("no free request slot for a fork")
+        room = self.options.ctx_size - len(source.prompt)
+        max_new = room if params.n_predict < 0 else min(params.n_predict, room)
+        if max_new <= n_output or not 0 <= n_keep < len(source.prompt) + n_output:
+            raise AdmissionError(f"a fork with {n_output} tokens of an answer of up to {max_new}, {n_keep} tokens in the cache")
+        self.cache.fork(source.request_id, request_id, n_keep)
+        req = Request(request_id, list(source.prompt), params, output=source.output[:n_output], num_computed=n_keep, state=RUNNING,
+                      max_new=max_new, arrival=next(self._arrivals), rng=XorShift64(params.seed))
+        self.running.append(req)
+        return req
 
     # ---- inner workings ----------------------------------------------------------------------------
     def _preempt(self, victim: Request) -> None:

@@ -224,9 +224,10 @@ def gemm_f32_tc(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optio
 def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, tok_req: torch.Tensor,
                   block_table: torch.Tensor, inv_freq: torch.Tensor, rot_half: int, mscale: float,
                   q_out: torch.Tensor, k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
-                  H: int, KV: int, dh: int, pair_layout: int = 0) -> None:
+                  H: int, KV: int, dh: int, pair_layout: int = 0, cache_rows: Optional[torch.Tensor] = None) -> None:
     """Rotates q and k of joined [q | k | v] rows and writes k, v into the request's pages. `pair_layout`: which
-    dimensions turn together, PAIRS_HALVES (j, j + rot_half) or PAIRS_INTERLEAVED (2j, 2j + 1)."""
+    dimensions turn together, PAIRS_HALVES (j, j + rot_half) or PAIRS_INTERLEAVED (2j, 2j + 1). `cache_rows` [T]: the cache row of each
+    token where it is not its position (drafted tokens)."""
     T = qkv.shape[0]
     _need(qkv, "qkv", torch.float32, (T, (H + 2 * KV) * dh))
     _need(positions, "positions", torch.int32, (T,)); _need(tok_req, "tok_req", torch.int32, (T,))
@@ -238,6 +239,12 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, tok_req: torch.Ten
         if k_cache.shape[1] != KV or k_cache.shape[3] != dh:
             raise KernelError(f"k_cache: shape {tuple(k_cache.shape)} does not hold {KV} heads of {dh}")
         page_size = k_cache.shape[2]
+    if cache_rows is not None:
+        _need(cache_rows, "cache_rows", torch.int32, (T,))
+        _call(_lib().bl_rope_kv_write_rows, _p(qkv), _p(positions), _p(cache_rows), _p(tok_req), _p(block_table),
+              block_table.shape[1], _p(inv_freq), rot_half, ctypes.c_float(mscale), _p(q_out), _p(k_cache),
+              _p(v_cache), _dt(q_out), T, H, KV, dh, page_size, pair_layout, _stream())
+        return
     _call(_lib().bl_rope_kv_write, _p(qkv), _p(positions), _p(tok_req), _p(block_table),
           block_table.shape[1], _p(inv_freq), rot_half, ctypes.c_float(mscale), _p(q_out), _p(k_cache),
           _p(v_cache), _dt(q_out), T, H, KV, dh, page_size, pair_layout, _stream())
@@ -959,9 +966,10 @@ def norm_inside_qkv(M: int, K: int) -> bool:
 def norm_qkv_rope(x: torch.Tensor, norm_w: torch.Tensor, eps: float, w_qkv: torch.Tensor, bias: Optional[torch.Tensor],
                   positions: torch.Tensor, tok_req: torch.Tensor, block_table: torch.Tensor, inv_freq: torch.Tensor,
                   mscale: float, q_out: torch.Tensor, k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
-                  H: int, KV: int, dh: int, pair_layout: int = 0) -> None:
+                  H: int, KV: int, dh: int, pair_layout: int = 0, cache_rows: Optional[torch.Tensor] = None) -> None:
     """rmsnorm -> joined q/k/v product (+ bias) -> rotation of q and k -> k, v into the pages, q out, in one launch (or, where
-    `norm_inside_qkv` says that the norm stays apart, in two)."""
+    `norm_inside_qkv` says that the norm stays apart, in two). `cache_rows` [M]: the cache row of each token where it is not its
+    position (drafted tokens)."""
     M, K = x.shape
     _need(x, "x", torch.float32); _need(norm_w, "norm_w", None, (K,)); _need(w_qkv, "w_qkv", torch.bfloat16, ((H + 2 * KV) * dh, K))
     _need(positions, "positions", torch.int32, (M,)); _need(tok_req, "tok_req", torch.int32, (M,))
@@ -975,12 +983,24 @@ def norm_qkv_rope(x: torch.Tensor, norm_w: torch.Tensor, eps: float, w_qkv: torc
         if k_cache.shape[1] != KV or k_cache.shape[3] != dh:
             raise KernelError(f"k_cache: shape {tuple(k_cache.shape)} does not hold {KV} heads of {dh}")
         page_size = k_cache.shape[2]
+    if cache_rows is not None:
+        _need(cache_rows, "cache_rows", torch.int32, (M,))
     if not norm_inside_qkv(M, K):
         normed = torch.empty((M, K), dtype=torch.bfloat16, device=x.device)
         rmsnorm(x, norm_w, eps, normed)
+        if cache_rows is not None:
+            _call(_lib().bl_qkv_rope_normed_rows, _p(normed), _p(w_qkv), _p(bias), _dt(bias) if bias is not None else 0, _p(positions),
+                  _p(cache_rows), _p(tok_req), _p(block_table), block_table.shape[1], _p(inv_freq), ctypes.c_float(mscale), _p(q_out),
+                  _p(k_cache), _p(v_cache), M, K, H, KV, dh, page_size, pair_layout, _stream())
+            return
         _call(_lib().bl_qkv_rope_normed, _p(normed), _p(w_qkv), _p(bias), _dt(bias) if bias is not None else 0, _p(positions),
               _p(tok_req), _p(block_table), block_table.shape[1], _p(inv_freq), ctypes.c_float(mscale), _p(q_out), _p(k_cache),
               _p(v_cache), M, K, H, KV, dh, page_size, pair_layout, _stream())
+        return
+    if cache_rows is not None:
+        _call(_lib().bl_norm_qkv_rope_rows, _p(x), _p(norm_w), _dt(norm_w), ctypes.c_float(eps), _p(w_qkv), _p(bias),
+              _dt(bias) if bias is not None else 0, _p(positions), _p(cache_rows), _p(tok_req), _p(block_table), block_table.shape[1],
+              _p(inv_freq), ctypes.c_float(mscale), _p(q_out), _p(k_cache), _p(v_cache), M, K, H, KV, dh, page_size, pair_layout, _stream())
         return
     _call(_lib().bl_norm_qkv_rope, _p(x), _p(norm_w), _dt(norm_w), ctypes.c_float(eps), _p(w_qkv), _p(bias),
           _dt(bias) if bias is not None else 0, _p(positions), _p(tok_req), _p(block_table), block_table.shape[1],

@@ -135,6 +135,10 @@ class Mixer(Part):
     # over the batch, no host reads): such a mixer may be captured in a CUDA graph and replayed.
     graph_safe = False
 
+    # True when forward() also runs steps of drafted trees (`ctx.tree_mask`, `ctx.cache_rows`): nodes that see their ancestors only, at
+    # positions of their own, and whose cached rows can be dropped or moved afterwards.
+    takes_trees = False
+
     def cache_spec(self):
         return None
 
@@ -177,6 +181,11 @@ class GQAAttention(Mixer):
     """
     graph_safe = True
     takes_pending_norm = True            # its first product can finish an RMS norm that the product before has begun
+
+    @property
+    def takes_trees(self) -> bool:
+        """(Not a part that replaces the attention or the whole forward pass: it would have to look at the trees itself.)"""
+        return type(self).attend is GQAAttention.attend and type(self).forward is GQAAttention.forward
 
     def takes_pending_norm_at(self, rows: int) -> bool:
         """... in steps with enough rows for the product on pairs of SMs (with few rows the norm is part of the q/k/v
@@ -236,7 +245,9 @@ class GQAAttention(Mixer):
             # many rows: bias, rotation and the writes of q, k and v are the epilogue of the joined product (and the
             # scale of a norm that the product before has begun)
             cs, sn = self.rotary.step_table(ctx)
-            ops.qkv_rope_tc(rows, self.w_qkv, self.b_qkv if self.qkv_bias else None, ctx.positions, ctx.tok_req, table, cs, sn,
+            # (the rotation is in the table: what this kernel calls positions are cache rows)
+            ops.qkv_rope_tc(rows, self.w_qkv, self.b_qkv if self.qkv_bias else None,
+                            ctx.positions if ctx.cache_rows is None else ctx.cache_rows, ctx.tok_req, table, cs, sn,
                             q, k_cache if write_cache else None, v_cache if write_cache else None, self.H, self.KV, self.dh,
                             row_sums=pending.sums if pending is not None else None, eps=pending.eps if pending is not None else 0.0)
         else:
@@ -246,7 +257,7 @@ class GQAAttention(Mixer):
             linear(ctx, h, self.w_qkv, qkv, self.b_qkv, EPI_BIAS if self.qkv_bias else EPI_NONE)
             ops.rope_kv_write(qkv, ctx.positions, ctx.tok_req, table, self.rotary.inv_freq, self.rotary.rot_half,
                               self.rotary.mscale, q, k_cache if write_cache else None,
-                              v_cache if write_cache else None, self.H, self.KV, self.dh, self.rotary.pair_layout)
+                              v_cache if write_cache else None, self.H, self.KV, self.dh, self.rotary.pair_layout, ctx.cache_rows)
         attn = ctx.empty((T, self.H * self.dh))
         self.attend(ctx, q, k_cache, v_cache, table, attn)
         self.project_out(ctx, attn, residual)
@@ -269,7 +280,7 @@ class GQAAttention(Mixer):
         ops.norm_qkv_rope(x, norm.weight, norm.eps, self.w_qkv, self.b_qkv if self.qkv_bias else None,
                           ctx.positions, ctx.tok_req, table, self.rotary.inv_freq, self.rotary.mscale, q,
                           k_cache if write_cache else None, v_cache if write_cache else None, self.H, self.KV, self.dh,
-                          self.rotary.pair_layout)
+                          self.rotary.pair_layout, ctx.cache_rows)
         attn = ctx.empty((T, self.H * self.dh))
         self.attend(ctx, q, k_cache, v_cache, table, attn)
         self.project_out(ctx, attn, x)
@@ -282,6 +293,9 @@ class GQAAttention(Mixer):
         return PLAN_KEY, attention_plan(q_lens, ctx_lens, filler)
 
     def attend(self, ctx, q, k_cache, v_cache, table, out):
+        if ctx.tree_mask is not None:
+            ops.attention_tree(q, k_cache, v_cache, ctx.cu_q, ctx.ctx_len, ctx.tree_mask, table, out, self.H, self.window, self.scale)
+            return
         paged_attention(ctx, q, k_cache, v_cache, table, out, self.H, self.KV, self.dh, self.window, self.scale)
 
 BUILT_HEAD_SIZES = (16, 32, 48, 64, 96, 128)        # head sizes of the tensor-core attention kernels

@@ -159,6 +159,10 @@ class StepContext:
     memo: dict = field(default_factory=dict)       # what a part works out once per step and its other layers reuse
     next_norm: object = None                       # the norm that reads the residual stream after the part that runs now (or None)
     norm_after_block: object = None                # ... after the block that runs now
+    # a step of drafted trees (`Mixer.takes_trees`): token t is a node that sees the nodes of `tree_mask[t]` (64 bits) of its request, lies in
+    # cache row `cache_rows[t]` and stands at `positions[t]`; a request's committed tokens are ctx_len[r] minus its nodes
+    tree_mask: Optional[torch.Tensor] = None
+    cache_rows: Optional[torch.Tensor] = None
     after_block: object = None                     # what a model wants done with the stream behind the block that runs now
                                                    # (`parts.depth.AfterBlock`); a block that can fold it into its last kernel does
 

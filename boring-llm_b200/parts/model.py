@@ -6,6 +6,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
+from ..cache import PagedKVSpec
 from ..weights import TensorSpec
 from .base import Part, takes_pending_norm
 
@@ -103,6 +104,12 @@ class DecoderModel(Part):
     def graph_safe(self) -> bool:
         """Whether a decode step of this model may be captured in a CUDA graph and replayed."""
         return all(getattr(b, "graph_safe", False) for b in self.blocks)
+
+    @property
+    def takes_trees(self) -> bool:
+        """Whether this model runs steps of drafted trees: every mixer does, and a request keeps nothing but pages."""
+        return (self.embedding_cache is None and all(getattr(getattr(b, "mixer", None), "takes_trees", False) for b in self.blocks)
+                and all(spec is None or isinstance(spec, PagedKVSpec) for spec in self.cache_specs()))
 
     def cache_specs(self) -> list:
         """What each cache layer needs, indexed by cache layer (None where unused)."""
