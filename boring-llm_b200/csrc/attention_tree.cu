@@ -204,7 +204,6 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
         cp_wait<0>();
         const bool whole = n_blocks == rq.nb;
         const size_t slot = 2 * (size_t)blockIdx.x + (first ? 0 : 1);
-        float* part = tree_outputs(p.scratch, gridDim.x) + slot * ROWS * p.dh;
         float* stats = tree_stats(p.scratch, gridDim.x, ROWS, p.dh) + slot * ROWS * 2;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
@@ -224,9 +223,12 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
         }
         if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 4 * NV; ++j) {
-                const int col = tx * 4 + 64 * (j >> 2) + (j & 3);
-                if (col < p.dh) *reinterpret_cast<float4*>(part + (size_t)col * ROWS + ty * 4) = make_float4(o[0][j], o[1][j], o[2][j], o[3][j]);
+            for (int v = 0; v < NV; ++v) {
+                if (tx * 4 + 64 * v >= dp) continue;
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *tree_cols(tree_outputs(p.scratch, gridDim.x), slot, ROWS, p.dh, ty * 4 + a, tx + 16 * v) =
+                        make_float4(o[a][4 * v], o[a][4 * v + 1], o[a][4 * v + 2], o[a][4 * v + 3]);
             }
         }
         left -= n_blocks;
@@ -283,7 +285,7 @@ extern "C" int bl_attention_tree(const void* q, const void* k_cache, const void*
     const int G = H / KV, blocks = resident_blocks(dh), npt = ROWS / G < TREE_MAX_NODES ? ROWS / G : TREE_MAX_NODES;
     if (!tree_line_fits(R, KV, npt, max_pages, page_size, KEYS) || blocks > TREE_MERGE_MAX)
         BL_FAIL("bl_attention_tree: %d requests with tables of %d pages of %d tokens are more work than a launch counts", R, max_pages, page_size);
-    const TreeLine line{cu_q, ctx_len, R, KV, window, npt};
+    const TreeLine line = tree_line(cu_q, ctx_len, R, KV, window, npt);
     const auto* mk = reinterpret_cast<const unsigned long long*>(mask);
     const float scale_log2 = scale * 1.4426950408889634f;
     if (dtype == BL_F32)

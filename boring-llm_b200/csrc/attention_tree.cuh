@@ -16,7 +16,11 @@ constexpr int TREE_MAX_NODES = 64;     // a node's view of its request's nodes i
 
 struct TreeLine {
     const int* cu_q; const int* ctx_len; int R, KV, window, npt;          // npt: nodes of a row tile
+    int inv_npt;                                                         // 65,536 / npt, rounded up: x / npt = x inv_npt >> 16 for x < 1,024
 };
+inline TreeLine tree_line(const int* cu_q, const int* ctx_len, int R, int KV, int window, int npt) {
+    return TreeLine{cu_q, ctx_len, R, KV, window, npt, (65536 + npt - 1) / npt};
+}
 // One request: n nodes behind c committed tokens; key blocks b0 .. b0 + nb - 1 hold what its nodes may see.
 struct TreeRequest { int begin, n, c, lo, tiles, b0, nb; };
 
@@ -28,7 +32,7 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeLine& a, int r) {
     q.c = a.ctx_len[r] - n;
     q.n = min(n, TREE_MAX_NODES);
     const bool none = n <= 0 || q.c < 0;                                 // a request without nodes has no part of the line
-    q.tiles = none ? 0 : (q.n + a.npt - 1) / a.npt;
+    q.tiles = none ? 0 : (q.n + a.npt - 1) * a.inv_npt >> 16;           // x < 128, npt <= 64: x (inv npt - 65,536) < 65,536
     q.lo = a.window > 0 ? max(0, q.c - a.window + 1) : 0;                // the first node's position is c
     q.b0 = q.lo / KEYS;
     q.nb = none ? 0 : (q.c + q.n - 1) / KEYS + 1 - q.b0;
@@ -155,12 +159,17 @@ __device__ __forceinline__ unsigned tree_bits(unsigned long long mask, int c, in
     return w;
 }
 
-// The scratch: a TreeCut per block, then 2 * blocks slots of [dh][rows] outputs (a thread has a row: neighbouring threads write neighbouring
-// words), then [2 * blocks][rows][2] maxima and sums. A block's first segment has slot 2 * block, one that it begins (and the next
+// The scratch: a TreeCut per block, then 2 * blocks slots of [dh / 4][rows][4] outputs (a thread has a row: neighbouring threads write
+// neighbouring 16 bytes; dh rounded up to fours), then [2 * blocks][rows][2] maxima and sums. A block's first segment has slot 2 * block, one that it begins (and the next
 // block goes on with) slot 2 * block + 1.
-__host__ __device__ __forceinline__ size_t tree_scratch_floats(int blocks, int rows, int dh) { return (size_t)8 * blocks + (size_t)2 * blocks * rows * (dh + 2); }
+__host__ __device__ __forceinline__ size_t tree_slot(int rows, int dh) { return (size_t)rows * ((dh + 3) & ~3); }
+__host__ __device__ __forceinline__ size_t tree_scratch_floats(int blocks, int rows, int dh) { return (size_t)8 * blocks + 2 * blocks * (tree_slot(rows, dh) + 2 * rows); }
 __device__ __forceinline__ float* tree_outputs(float* scratch, int blocks) { return scratch + (size_t)8 * blocks; }
-__device__ __forceinline__ float* tree_stats(float* scratch, int blocks, int rows, int dh) { return scratch + (size_t)8 * blocks + (size_t)2 * blocks * rows * dh; }
+__device__ __forceinline__ float* tree_stats(float* scratch, int blocks, int rows, int dh) { return scratch + (size_t)8 * blocks + 2 * blocks * tree_slot(rows, dh); }
+// Columns 4 c4 .. of a row
+__device__ __forceinline__ float4* tree_cols(float* outputs, size_t slot, int rows, int dh, int row, int c4) {
+    return reinterpret_cast<float4*>(outputs + slot * tree_slot(rows, dh)) + (size_t)c4 * rows + row;
+}
 
 template <typename TT>
 struct TreeMerge { float* scratch; TT* out; int blocks, dh, H, G; };
@@ -169,22 +178,22 @@ constexpr int TREE_MERGE_WARPS = 8, TREE_MERGE_MAX = 1024;               // most
 constexpr int TREE_MERGE_MANY = 8;                                       // more parts than this: four blocks share 32 rows
 
 // o = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k over the parts k of each unit that is cut, in their order. The blocks share the rows of all
-// cut units out, 32 at a time: lane = row, a warp has NC columns (of a unit with many parts, as when one long request is on all SMs, NC
-// / 4 of them), and the finished rows leave through shared memory.
+// cut units out, 32 at a time: lane = row, a warp has NC columns (of a unit with many parts, as when one long request is on all SMs, a
+// quarter of them, four at least), and the finished rows leave through shared memory.
 template <int ROWS, int NC, typename TT>
 struct TreeMergeTile {
     template <int COLS>
     static __device__ __forceinline__ void run(const TreeMerge<TT>& p, const TreeCut& cut, int row0, int col_first, float* tile) {
         constexpr int LD = TREE_MERGE_WARPS * COLS + 1;
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = cut.nodes * p.G, row = row0 + lane, col0 = col_first + warp * COLS;
-        const float* outs = tree_outputs(p.scratch, p.blocks);
+        float* outs = tree_outputs(p.scratch, p.blocks);
         const float* stats = tree_stats(p.scratch, p.blocks, ROWS, p.dh);
         const bool live = row < rows;
         float m = -INFINITY, l = 0.f, o[COLS] = {};
-        constexpr int AHEAD = COLS <= 8 ? 4 : 2;                         // parts whose numbers are asked for together
+        constexpr int AHEAD = COLS <= 4 ? 8 : COLS <= 8 ? 4 : 2;                         // parts whose numbers are asked for together
         for (int k0 = 0; k0 < cut.parts; k0 += AHEAD) {
             float2 ml[AHEAD];
-            float v[AHEAD][COLS];
+            float4 v[AHEAD][COLS / 4];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int k = k0 + u;
@@ -192,7 +201,8 @@ struct TreeMergeTile {
                 const size_t slot = k == 0 ? cut.first : cut.slot + 2 * (k - 1);
                 ml[u] = there ? *reinterpret_cast<const float2*>(stats + 2 * (slot * ROWS + row)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) v[u][j] = there && col0 + j < p.dh ? outs[(slot * p.dh + col0 + j) * ROWS + row] : 0.f;
+                for (int j = 0; j < COLS; j += 4)
+                    v[u][j / 4] = there && col0 + j < p.dh ? *tree_cols(outs, slot, ROWS, p.dh, row, (col0 + j) / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {                            // one part more, against the larger of the two maxima
@@ -201,7 +211,10 @@ struct TreeMergeTile {
                 m = top;
                 l = l * a + ml[u].y * b;
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) o[j] = o[j] * a + v[u][j] * b;
+                for (int j = 0; j < COLS; j += 4) {
+                    o[j] = o[j] * a + v[u][j / 4].x * b; o[j + 1] = o[j + 1] * a + v[u][j / 4].y * b;
+                    o[j + 2] = o[j + 2] * a + v[u][j / 4].z * b; o[j + 3] = o[j + 3] * a + v[u][j / 4].w * b;
+                }
             }
         }
         const float inv = l > 0.f ? 1.0f / l : 0.f;
@@ -221,11 +234,12 @@ template <int ROWS, int NC, typename TT>
 __global__ void __launch_bounds__(32 * TREE_MERGE_WARPS) tree_merge_kernel(const TreeMerge<TT> p) {
     __shared__ float tile[32 * (TREE_MERGE_WARPS * NC + 1)];
     __shared__ int upto[TREE_MERGE_MAX], warp_sum[TREE_MERGE_WARPS];     // items of the cuts up to each
+    constexpr int MANY = NC > 8 ? NC / 4 : 4, SHARE = NC / MANY;         // of a unit with many parts
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     bl_pdl_wait();
     bl_pdl_trigger();
     const TreeCut* cuts = reinterpret_cast<const TreeCut*>(p.scratch);
-    auto items_of = [&](int parts, int nodes) { return parts == 0 ? 0 : (nodes * p.G + 31) / 32 * (parts > TREE_MERGE_MANY ? 4 : 1); };
+    auto items_of = [&](int parts, int nodes) { return parts == 0 ? 0 : (nodes * p.G + 31) / 32 * (parts > TREE_MERGE_MANY ? SHARE : 1); };
     int total = 0;
     for (int i0 = 0; i0 < p.blocks; i0 += 32 * TREE_MERGE_WARPS) {
         int mine = i0 + tid < p.blocks ? items_of(cuts[i0 + tid].parts, cuts[i0 + tid].nodes) : 0;
@@ -250,7 +264,7 @@ __global__ void __launch_bounds__(32 * TREE_MERGE_WARPS) tree_merge_kernel(const
             if (at + half <= p.blocks && upto[at + half - 1] <= item) at += half;
         const TreeCut cut = cuts[at];
         const int nth = item - (upto[at] - items_of(cut.parts, cut.nodes));
-        if (cut.parts > TREE_MERGE_MANY) TreeMergeTile<ROWS, NC, TT>::template run<NC / 4>(p, cut, nth / 4 * 32, nth % 4 * (TREE_MERGE_WARPS * NC / 4), tile);
+        if (cut.parts > TREE_MERGE_MANY) TreeMergeTile<ROWS, NC, TT>::template run<MANY>(p, cut, nth / SHARE * 32, nth % SHARE * (TREE_MERGE_WARPS * MANY), tile);
         else TreeMergeTile<ROWS, NC, TT>::template run<NC>(p, cut, nth * 32, 0, tile);
     }
 }

@@ -103,6 +103,20 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :: "memory");
 }
+// 16 columns, and the wait for all loads, tied to what they bring
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_arrived(uint32_t (&a)[16], uint32_t (&b)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                   "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]) :: "memory");
+    asm volatile("" : "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]),
+                      "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15]) :: "memory");
+}
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -203,8 +217,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // work of a segment is a row of tasks: with two tiles, both tiles on key block 0, both on key block 1, ..; with one, the key
     // blocks. Tasks alternate between the groups of row warps throughout the kernel: the task's number decides the group (mod 2) and the
     // buffer of scores (mod SBUFS).
-    auto segments = [&](auto f, bool to_the_end = false) {
-        for (int seg = 0; (ok || to_the_end) && left > 0; ++seg) {
+    auto segments = [&](auto f) {
+        for (int seg = 0; ok && left > 0; ++seg) {
             const int n = min(left, w.q.b0 + w.q.nb - w.b);
             f(seg, n, w.q.n - w.tile * p.line.npt > p.npt && p.line.npt > p.npt);
             left -= n;
@@ -352,18 +366,25 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             return fine;
         };
         ok = __all_sync(0xffffffffu, ok);
-        segments([&](int seg, int n, bool two) {
+        // What a row may see, asked for ahead: the mask of the node that this thread's row has in the unit at `u` (0: the tile has no such row).
+        auto is_two = [&](const TreePlace& u) { return u.q.n - u.tile * p.line.npt > p.npt && p.line.npt > p.npt; };
+        auto ask_mask = [&](const TreePlace& u, int tasks_before) -> unsigned long long {
+            const int tile = is_two(u) ? (tasks_before & 1) ^ grp : 0, at = u.tile * p.line.npt + tile * p.npt;
+            return left > 0 && node < min(p.npt, u.q.n - at) ? p.mask[(size_t)u.q.begin + at + node] : 0;
+        };
+        unsigned long long node_mask = ask_mask(w, 0);
+        for (int seg = 0; left > 0; ++seg) {                             // (a warp that has given up still comes to the groups' barriers)
             const TreeRequest q = w.q;
+            const int n = min(left, q.b0 + q.nb - w.b);
+            const bool two = is_two(w);
             const int first = (done & 1) ^ grp;                          // this group's first task of the segment
             const int tile = two ? first : 0, node0 = w.tile * p.line.npt + tile * p.npt, nodes = min(p.npt, q.n - node0), hi = q.c + q.n - 1;
             const bool valid = node < nodes, warp_rows = (warp & 3) * 32 < nodes * p.G;
-            const size_t tok = (size_t)q.begin + node0 + node;
             unsigned long long seen = 0;
             int lo = q.c;                                                // a row that the tile does not have sees nothing that matters
             if (valid) {
-                const unsigned long long m = p.mask[tok];
-                const int pos = q.c + max(__popcll(q.n < 64 ? m & ((1ULL << q.n) - 1) : m) - 1, 0);
-                seen = tree_mask(m, q.n, p.line.window);
+                const int pos = q.c + max(__popcll(q.n < 64 ? node_mask & ((1ULL << q.n) - 1) : node_mask) - 1, 0);
+                seen = tree_mask(node_mask, q.n, p.line.window);
                 lo = p.line.window > 0 ? min(max(0, pos - p.line.window + 1), q.c) : 0;
             }
             float m = -INFINITY, l = 0.f;
@@ -459,6 +480,12 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             done += tasks;
             behind += n;
+            left -= n;
+            TreePlace next = w;                                          // the next unit and its mask arrive during the outputs
+            if (left > 0) {
+                tree_next_unit<KEYS>(p.line, next);
+                node_mask = ask_mask(next, done);
+            }
             // the segment's outputs (against m, not divided by l yet), once the group's last product has been added
             const bool whole = n == q.nb, had = tasks > first;
             ok = ok && (!had || product_done(13));
@@ -482,22 +509,23 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             w_own *= inv; w_other *= inv;
             const size_t slot = 2 * (size_t)blockIdx.x + (seg == 0 ? 0 : 1);
             const int unit_row = tile * p.npt * p.G + row;
-            float* part = tree_outputs(p.scratch, gridDim.x) + slot * UNIT_ROWS * DH + unit_row;
+            float4* part = tree_cols(tree_outputs(p.scratch, gridDim.x), slot, UNIT_ROWS, DH, unit_row, 0);
             auto out_row = [&](int r) { return p.out + (((size_t)q.begin + node0 + r / p.G) * p.H + w.kvh * p.G + r % p.G) * DH; };
             __nv_bfloat16 *dst_even = out_row(row & ~1), *dst_odd = out_row(row | 1);
             const bool valid_even = (row & ~1) < nodes * p.G, valid_odd = (row | 1) < nodes * p.G;
             if (ok && warp_rows) {
-#pragma unroll 1
-                for (int h = h0; h < h1; ++h) {
-                    uint32_t v[16];
+                // sixteen columns at a time, the next ones on their way meanwhile
+                uint32_t own_a[16], other_a[16], own_b[16], other_b[16];
+                auto ask = [&](uint32_t (&own16)[16], uint32_t (&other16)[16], int h) {
+                    if (had) tmem_ld16(t_o + h * 16, own16);
+                    if (other) tmem_ld16(t_other + h * 16, other16);
+                };
+                auto emit = [&](uint32_t (&own16)[16], uint32_t (&other16)[16], int h) {
                     float f[16];
-                    if (had) tmem_ld16_wait(t_o + h * 16, v);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) f[x] = had ? __uint_as_float(v[x]) * w_own : 0.f;
-                    if (other) {
-                        tmem_ld16_wait(t_other + h * 16, v);
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) f[x] = fmaf(__uint_as_float(v[x]), w_other, f[x]);
+                    for (int x = 0; x < 16; ++x) {
+                        f[x] = had ? __uint_as_float(own16[x]) * w_own : 0.f;
+                        if (other) f[x] = fmaf(__uint_as_float(other16[x]), w_other, f[x]);
                     }
                     if (whole) {
                         // 32 bytes of a row leave together: neighbouring lanes exchange halves, so that both write the even lane's row, then the odd one's
@@ -516,8 +544,19 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (odd ? valid : valid_odd) *reinterpret_cast<uint4*>(dst_odd + h * 16 + (odd ? 8 : 0)) = odd ? own_half : other_half;
                     } else if (valid) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) part[(size_t)(h * 16 + x) * UNIT_ROWS] = f[x];
+                        for (int x = 0; x < 16; x += 4) part[(size_t)(h * 4 + x / 4) * UNIT_ROWS] = make_float4(f[x], f[x + 1], f[x + 2], f[x + 3]);
                     }
+                };
+                ask(own_a, other_a, h0);
+#pragma unroll 1
+                for (int h = h0; h < h1; h += 2) {                       // (a group has an even number of sixteens)
+                    tmem_ld16_arrived(own_a, other_a);
+                    ask(own_b, other_b, h + 1);
+                    emit(own_a, other_a, h);
+                    __syncwarp();
+                    tmem_ld16_arrived(own_b, other_b);
+                    if (h + 2 < h1) ask(own_a, other_a, h + 2);
+                    emit(own_b, other_b, h + 1);
                     __syncwarp();
                 }
             }
@@ -525,7 +564,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 *reinterpret_cast<float2*>(tree_stats(p.scratch, gridDim.x, UNIT_ROWS, DH) + (slot * UNIT_ROWS + unit_row) * 2) = make_float2(m, l);
             fence_before_sync();                                         // the outputs have been read: the next unit's first products may write them
             if (!two) asm volatile("bar.sync 1, 256;" ::: "memory");
-        }, true);                                                        // (a warp that has given up still comes to the groups' barriers)
+            w = next;
+        }
     }
     fence_before_sync();
     __syncthreads();
@@ -562,11 +602,9 @@ int launch(const void* q, const void* k_cache, const void* v_cache, const Params
     }
     BL_CUDA(bl_launch_dependent(attention_tree_tc_kernel<S>, dim3(blocks), dim3(THREADS), (size_t)S::SMEM_BYTES, stream, mq, mk, mv, p));
     BL_CHECK_LAUNCH("bl_attention_tree_tc");
-    {
-        TreeMerge<__nv_bfloat16> mg{p.scratch, p.out, blocks, S::DH, p.H, p.G};
-        BL_CUDA(bl_launch_dependent(tree_merge_kernel<UNIT_ROWS, S::DH / 8, __nv_bfloat16>, dim3(4 * blocks), dim3(32 * TREE_MERGE_WARPS), 0, stream, mg));
-        BL_CHECK_LAUNCH("bl_attention_tree_tc (merge)");
-    }
+    TreeMerge<__nv_bfloat16> mg{p.scratch, p.out, blocks, S::DH, p.H, p.G};
+    BL_CUDA(bl_launch_dependent(tree_merge_kernel<UNIT_ROWS, S::DH / 8, __nv_bfloat16>, dim3(4 * blocks), dim3(32 * TREE_MERGE_WARPS), 0, stream, mg));
+    BL_CHECK_LAUNCH("bl_attention_tree_tc (merge)");
     return 0;
 }
 
@@ -593,7 +631,7 @@ extern "C" int bl_attention_tree_tc(const void* q, const void* k_cache, const vo
     const int unit = 2 * npt < TREE_MAX_NODES ? 2 * npt : TREE_MAX_NODES;
     if (!tree_line_fits(R, KV, unit, max_pages, PAGE, KEYS) || bl_device_sms() > TREE_MERGE_MAX)
         BL_FAIL("%s: %d requests with tables of %d pages are more work than a launch counts", WHO, R, max_pages);
-    Params p{TreeLine{cu_q, ctx_len, R, KV, window, unit}, (__nv_bfloat16*)out, reinterpret_cast<const unsigned long long*>(mask), block_table, max_pages,
+    Params p{tree_line(cu_q, ctx_len, R, KV, window, unit), (__nv_bfloat16*)out, reinterpret_cast<const unsigned long long*>(mask), block_table, max_pages,
              H, G, npt, n_pages * KV * 2, scale * 1.4426950408889634f, scratch};
     if (dh == 64) return launch<Shape<64>>(q, k_cache, v_cache, p, T, bl_device_sms(), (cudaStream_t)stream);
     return launch<Shape<128>>(q, k_cache, v_cache, p, T, bl_device_sms(), (cudaStream_t)stream);
