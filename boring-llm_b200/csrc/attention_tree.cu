@@ -32,7 +32,7 @@ __device__ __forceinline__ void cp16(float* dst, const float* src, bool there) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
-// 64 rows of dh values (row i at src + offs[i], offs < 0: zeros) into shared rows of `ld` floats, of which the last dp - dh are zeros.
+// 64 rows of dh values (row i at src + offs[i], offs < 0: zeros; rows of q, keys or values) into shared rows of `ld` floats, of which the last dp - dh are zeros.
 template <typename TT, bool VEC>
 __device__ __forceinline__ void copy_rows(float* dst, int ld, const TT* src, const long long* offs, int dh, int dp) {
     const int pieces = dp >> 2;
@@ -59,7 +59,7 @@ __device__ __forceinline__ void copy_rows(float* dst, int ld, const TT* src, con
 template <typename TT, bool VEC, int NV>
 __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kernel(const Params<TT> p) {
     extern __shared__ __align__(16) float sm[];
-    __shared__ long long offs[2][KEYS];                                  // where the keys of this block and the next lie
+    __shared__ long long offs[2][KEYS], q_offs[ROWS];                    // where the keys of this block and the next lie, and the rows of q
     __shared__ TreeShare s_share;
     __shared__ int s_ends[32];
     const int dp = (p.dh + 3) & ~3, ld = dp + 4;
@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
     bl_pdl_wait();
     bl_pdl_trigger();
     if (tid < 32) {
-        const TreeShare s = tree_share<KEYS, 1, 0>(p.line, gridDim.x, blockIdx.x, s_ends);
+        TreeShare s = tree_share<KEYS, 1, 0>(p.line, gridDim.x, blockIdx.x, s_ends);
         if (tid == 0) {
             s_share = s;
+            s.cut.items = tree_merge_items(s.cut, p.G, 8 * NV);
             reinterpret_cast<TreeCut*>(p.scratch)[blockIdx.x] = s.cut;
         }
     }
@@ -99,12 +100,14 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
         // the tile's rows of q, and what each of this thread's four rows may see
         __syncthreads();                                                 // the segment before has been read
         place(w.b, 0);
-        for (int i = tid; i < ROWS * (dp >> 2); i += THREADS) {
-            const int row = i / (dp >> 2), d = (i - row * (dp >> 2)) << 2, node = row / p.G;
-            const TT* src = p.q + ((size_t)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) qs[row * ld + d + j] = node < nodes && d + j < p.dh ? bl_load(src + d + j) : 0.f;
+        if (tid >= KEYS && tid < KEYS + ROWS) {
+            const int row = tid - KEYS, node = row / p.G;
+            q_offs[row] = node < nodes ? ((long long)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh : -1;
         }
+        __syncthreads();
+        copy_rows<TT, VEC>(qs, ld, p.q, q_offs, p.dh, dp);               // q and the first keys arrive together
+        copy_rows<TT, VEC>(ks, ld, p.kc, offs[0], p.dh, dp);
+        const bool rows_here = (tid >> 5) * 8 < nodes * p.G;             // a warp has eight rows: without one it only copies
         unsigned long long seen[4];
         int lo[4];
 #pragma unroll
@@ -125,8 +128,6 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
 #pragma unroll
             for (int j = 0; j < 4 * NV; ++j) o[a][j] = 0.f;
         }
-        __syncthreads();
-        copy_rows<TT, VEC>(ks, ld, p.kc, offs[0], p.dh, dp);
         for (int i = 0; i < n_blocks; ++i) {
             const int k0 = (w.b + i) * KEYS, buf = i & 1;
             copy_rows<TT, VEC>(vs, ld, p.vc, offs[buf], p.dh, dp);       // (behind the barrier that ends the block before)
@@ -138,7 +139,8 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
             for (int a = 0; a < 4; ++a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[a][j] = 0.f;
-            for (int d = 0; d < dp; d += 4) {
+#pragma unroll 2
+            for (int d = 0; rows_here && d < dp; d += 4) {
                 float4 qa[4], kb[4];
 #pragma unroll
                 for (int a = 0; a < 4; ++a) qa[a] = *reinterpret_cast<const float4*>(qs + (ty * 4 + a) * ld + d);
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
             __syncthreads();                                             // keys have been read
             if (i + 1 < n_blocks) copy_rows<TT, VEC>(ks, ld, p.kc, offs[buf ^ 1], p.dh, dp);
             else cp_commit();
+            if (rows_here) {
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 float top = -INFINITY;
@@ -181,9 +184,11 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<float4*>(ps + (tx + 16 * j) * LDP + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+            }
             cp_wait<1>();
             __syncthreads();                                             // values and P are there
-            for (int j = 0; j < KEYS; ++j) {
+#pragma unroll 4
+            for (int j = 0; rows_here && j < KEYS; ++j) {
                 const float4 pr = *reinterpret_cast<const float4*>(ps + j * LDP + ty * 4);
 #pragma unroll
                 for (int v = 0; v < NV; ++v) {
@@ -262,7 +267,7 @@ int launch(const Params<TT>& p, int blocks, cudaStream_t s) {
 
 template <typename TT>
 int run(Params<TT> p, int blocks, cudaStream_t s) {
-    const bool vec = p.dh % 4 == 0 && (((uintptr_t)p.kc | (uintptr_t)p.vc) & (sizeof(TT) * 4 - 1)) == 0;
+    const bool vec = p.dh % 4 == 0 && (((uintptr_t)p.q | (uintptr_t)p.kc | (uintptr_t)p.vc) & (sizeof(TT) * 4 - 1)) == 0;
     if (p.dh <= 64) return vec ? launch<TT, true, 1>(p, blocks, s) : launch<TT, false, 1>(p, blocks, s);
     if (p.dh <= 128) return vec ? launch<TT, true, 2>(p, blocks, s) : launch<TT, false, 2>(p, blocks, s);
     return vec ? launch<TT, true, 4>(p, blocks, s) : launch<TT, false, 4>(p, blocks, s);

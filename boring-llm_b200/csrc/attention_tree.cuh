@@ -56,7 +56,7 @@ __device__ __forceinline__ void tree_next_unit(const TreeLine& a, TreePlace& p) 
 }
 
 // A unit that the beginning of a part cuts, and no part before it: what the merge needs to know. parts = 0: there is none.
-struct TreeCut { int parts, first, slot, tok, nodes, kvh, pad0, pad1; };          // slots: first, then slot, slot + 2, .. (parts - 1 of them)
+struct TreeCut { int parts, first, slot, tok, nodes, kvh, items, pad; };           // slots: first, then slot, slot + 2, .. (parts - 1 of them)
 // A block's part of the line: `left` key blocks from `place` on (0: none), and what there is to merge at its beginning.
 struct TreeShare { TreePlace place; int left; TreeCut cut; };
 
@@ -174,8 +174,13 @@ __device__ __forceinline__ float4* tree_cols(float* outputs, size_t slot, int ro
 template <typename TT>
 struct TreeMerge { float* scratch; TT* out; int blocks, dh, H, G; };
 
-constexpr int TREE_MERGE_WARPS = 8, TREE_MERGE_MAX = 1024;               // most blocks of a launch whose units are merged
-constexpr int TREE_MERGE_MANY = 8;                                       // more parts than this: four blocks share 32 rows
+constexpr int TREE_MERGE_WARPS = 8, TREE_MERGE_MAX = 320;                // blocks of the attention's grid, at most
+constexpr int TREE_MERGE_MANY = 8;                                       // more parts than this: several blocks share 32 rows
+// Columns of a merging warp, of NC at few parts, and the blocks that share 32 rows then.
+__host__ __device__ constexpr int tree_merge_cols(int nc) { return nc > 8 ? nc / 4 : 4; }
+__device__ __forceinline__ int tree_merge_items(const TreeCut& cut, int G, int nc) {
+    return cut.parts == 0 ? 0 : (cut.nodes * G + 31) / 32 * (cut.parts > TREE_MERGE_MANY ? nc / tree_merge_cols(nc) : 1);
+}
 
 // o = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k over the parts k of each unit that is cut, in their order. The blocks share the rows of all
 // cut units out, 32 at a time: lane = row, a warp has NC columns (of a unit with many parts, as when one long request is on all SMs, a
@@ -232,38 +237,34 @@ struct TreeMergeTile {
 
 template <int ROWS, int NC, typename TT>
 __global__ void __launch_bounds__(32 * TREE_MERGE_WARPS) tree_merge_kernel(const TreeMerge<TT> p) {
+    constexpr int MANY = tree_merge_cols(NC), SHARE = NC / MANY, EACH = TREE_MERGE_MAX / 32;
     __shared__ float tile[32 * (TREE_MERGE_WARPS * NC + 1)];
-    __shared__ int upto[TREE_MERGE_MAX], warp_sum[TREE_MERGE_WARPS];     // items of the cuts up to each
-    constexpr int MANY = NC > 8 ? NC / 4 : 4, SHARE = NC / MANY;         // of a unit with many parts
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31;
     bl_pdl_wait();
     bl_pdl_trigger();
+    // Each warp looks through the cuts for itself (lane l at cuts l * per ..): one load, no barrier.
     const TreeCut* cuts = reinterpret_cast<const TreeCut*>(p.scratch);
-    auto items_of = [&](int parts, int nodes) { return parts == 0 ? 0 : (nodes * p.G + 31) / 32 * (parts > TREE_MERGE_MANY ? SHARE : 1); };
-    int total = 0;
-    for (int i0 = 0; i0 < p.blocks; i0 += 32 * TREE_MERGE_WARPS) {
-        int mine = i0 + tid < p.blocks ? items_of(cuts[i0 + tid].parts, cuts[i0 + tid].nodes) : 0;
+    const int per = (p.blocks + 31) / 32;
+    int items[EACH], mine = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, mine, o);
-            if (lane >= o) mine += v;
-        }
-        if (lane == 31) warp_sum[warp] = mine;
-        __syncthreads();
-        int before = total;
-        for (int w = 0; w < TREE_MERGE_WARPS; ++w) {
-            if (w < warp) before += warp_sum[w];
-            total += warp_sum[w];
-        }
-        if (i0 + tid < p.blocks) upto[i0 + tid] = before + mine;
-        __syncthreads();
+    for (int x = 0; x < EACH; ++x) items[x] = x < per && lane * per + x < p.blocks ? cuts[lane * per + x].items : 0;
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) mine += items[x];
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
     }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
-        int at = 0;                                                      // the first cut whose items reach beyond this one
-        for (int half = TREE_MERGE_MAX / 2; half > 0; half >>= 1)
-            if (at + half <= p.blocks && upto[at + half - 1] <= item) at += half;
-        const TreeCut cut = cuts[at];
-        const int nth = item - (upto[at] - items_of(cut.parts, cut.nodes));
+        const int src = __ffs(__ballot_sync(0xffffffffu, upto > item)) - 1;
+        int nth = item - (upto - mine), at = 0;                          // the lane that holds it finds its cut
+#pragma unroll
+        for (int x = 0; x < EACH; ++x)
+            if (at == x && nth >= items[x]) { nth -= items[x]; ++at; }
+        nth = __shfl_sync(0xffffffffu, nth, src);
+        const TreeCut cut = cuts[__shfl_sync(0xffffffffu, lane * per + at, src)];
         if (cut.parts > TREE_MERGE_MANY) TreeMergeTile<ROWS, NC, TT>::template run<MANY>(p, cut, nth / SHARE * 32, nth % SHARE * (TREE_MERGE_WARPS * MANY), tile);
         else TreeMergeTile<ROWS, NC, TT>::template run<NC>(p, cut, nth * 32, 0, tile);
     }

@@ -200,9 +200,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     bl_pdl_wait();
     bl_pdl_trigger();
     if (warp == 0) {
-        const TreeShare s = tree_share<KEYS, 4, 2>(p.line, gridDim.x, blockIdx.x, s_ends);
+        TreeShare s = tree_share<KEYS, 4, 2>(p.line, gridDim.x, blockIdx.x, s_ends);
         if (lane == 0) {
             *s_share = s;
+            s.cut.items = tree_merge_items(s.cut, p.G, DH / 8);
             reinterpret_cast<TreeCut*>(p.scratch)[blockIdx.x] = s.cut;
         }
     }
