@@ -47,6 +47,7 @@ class Engine:
             raise ValueError("draft_tokens: this model's mixers keep state of their own beside pages, or attend in a way of their own; "
                              "drafted tokens could not be taken back")
         self._ids = itertools.count()
+        self._early: List[Request] = []       # finished when a fork read the step ahead: the next step returns them
         self._inflight = None                 # (scheduled step, PendingDecode): launched, tokens not read yet
         self.stats_time = {"engine_steps": 0, "step_seconds": 0.0}
 
@@ -83,6 +84,11 @@ class Engine:
         step behind, and the GPU does not wait for the host between steps. A request that ends with an end token
         has then already got a row in the step after; that row's result is dropped (the reference's loop,
         src/model.br:2293-2304, feeds no token after the end token either: nothing of the row is kept)."""
+        done = self._step()
+        early, self._early = self._early, []
+        return early + done
+
+    def _step(self) -> List[Request]:
         t0 = time.perf_counter()
         if self._inflight is None:
             sched = self.scheduler.schedule()
@@ -142,7 +148,7 @@ class Engine:
     def fork(self, request, params: Optional[SamplingParams] = None, request_id=None) -> Request:
         """A second running request that goes on from where `request` (a `Request` that runs, its prompt computed) is, with parameters
         and a generator of its own. The pages of what both have in common are shared."""
-        self.drain()
+        self._early += self.drain()
         if request.state != RUNNING or request.remaining != 1:
             raise ValueError(f"request {request.request_id!r} cannot be forked: it has ended, or its prompt is not computed yet")
         return self._fork(request, params if params is not None else copy.copy(request.params), request_id, request.num_computed,
@@ -226,8 +232,11 @@ class Engine:
                 else:
                     reqs[at] = self.add_request(prompt, params)
             waiting = left
-            if waiting:
-                self.step()
+            if waiting and not self.step() and not self.scheduler.running:
+                # nothing runs and the sources cannot start: wait with them
+                for _, prompt, params, at in waiting:
+                    reqs[at] = self.add_request(prompt, params)
+                break
         self.run_until_done()
         return [list(r.output) for r in reqs]
 

@@ -605,6 +605,7 @@ class ModelRunner:
         if not entries:
             raise StepError("a step needs at least one entry")
         if self.options.debug_poison:
+            self.storage.copy_pages()                  # (a page may have been given back since it became a copy's source)
             self.storage.poison_freed_pages()
         if self._prepare_decode(entries):
             return None
@@ -853,6 +854,7 @@ class ModelRunner:
         if any(n > f for n, f in zip(need, free)):
             raise OutOfPages(f"the step needs {need} pages per group, {free} are free")
         if self.options.debug_poison:
+            self.storage.copy_pages()
             self.storage.poison_freed_pages()
         for e in entries:
             self.cache.reserve(e.request_id, len(e.tokens))

@@ -2199,14 +2199,24 @@ def hyper_step(x: torch.Tensor, n: int, x_out: Optional[torch.Tensor] = None, wr
 TREE_MAX_NODES = 64       # nodes of one request in a step: what a node sees of them is a 64-bit mask
 
 
-def _here(*tensors: torch.Tensor) -> None:
-    """All on the current CUDA device, whose current stream the kernels are launched on."""
-    devices = {t.get_device() for t in tensors}
-    if -1 in devices:
+def _here(first: torch.Tensor, *others: torch.Tensor) -> int:
+    """All on the current CUDA device. Returns its current stream, which the kernels are launched on."""
+    device = first.get_device()
+    for t in others:
+        if t.get_device() != device:
+            raise KernelError(f"tensors lie on {first.device} and {t.device}")
+    if device < 0:
         raise KernelError("must be CUDA tensors")
     now = torch.cuda.current_device() if _raw_device is None else _raw_device()
-    if devices != {now}:
-        raise KernelError(f"tensors lie on devices {sorted(devices)}, the current device is {now}")
+    if device != now:
+        raise KernelError(f"tensors lie on device {device}, the current device is {now}")
+    return _stream().value if _raw_stream is None else _raw_stream(device)
+
+
+def _list(t: torch.Tensor, name: str, dtype, n: int) -> None:
+    """A contiguous list of n numbers."""
+    if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or not t.is_contiguous():
+        _fits(t, name, dtype, (n,))
 
 
 def _fits(t: torch.Tensor, name: str, dtype, shape) -> None:
@@ -2239,7 +2249,7 @@ def _typed(name: str):
 def _tree_step(mask: torch.Tensor, cu_q: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor):
     """(T, R) of a step with trees."""
     T, R = mask.shape[0], ctx_len.shape[0]
-    _fits(mask, "mask", torch.int64, (T,)); _fits(cu_q, "cu_q", torch.int32, (R + 1,)); _fits(ctx_len, "ctx_len", torch.int32, (R,))
+    _list(mask, "mask", torch.int64, T); _list(cu_q, "cu_q", torch.int32, R + 1); _list(ctx_len, "ctx_len", torch.int32, R)
     if block_table.dim() != 2 or block_table.shape[0] < R:
         raise KernelError(f"block_table: must have a row for each of the {R} requests, got {tuple(block_table.shape)}")
     if block_table.dtype is not torch.int32 or not block_table.is_contiguous():
@@ -2262,20 +2272,21 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if k_cache.dim() != 4:
         raise KernelError(f"k_cache: must be [pages, kv heads, page size, head size], got {tuple(k_cache.shape)}")
     _, KV, page_size, dh = k_cache.shape
-    if H <= 0 or H % KV != 0:
+    if H <= 0 or KV <= 0 or H % KV != 0:
         raise KernelError(f"{H} heads cannot share {KV} key/value heads")
+    window = min(window, 0x7fffffff)
     _dt(q)
     _fits(q, "q", q.dtype, (T, H * dh)); _fits(k_cache, "k_cache", q.dtype, k_cache.shape)
     _fits(v_cache, "v_cache", q.dtype, k_cache.shape); _fits(out, "out", q.dtype, (T, H * dh))
-    _here(q, k_cache, v_cache, cu_q, ctx_len, mask, block_table, out)
+    stream = _here(q, k_cache, v_cache, cu_q, ctx_len, mask, block_table, out)
     ptr_q, ptr_k, ptr_v, ptr_out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     tc = q.dtype is torch.bfloat16 and (ptr_q | ptr_k | ptr_v | ptr_out) % 16 == 0 and _tree_tc_built(H, KV, dh, page_size)
     scratch = torch.empty(_tree_scratch(dh, tc), dtype=torch.float32, device=q.device)
     rest = (cu_q.data_ptr(), ctx_len.data_ptr(), mask.data_ptr(), block_table.data_ptr(), block_table.shape[1], ptr_out, scratch.data_ptr(), T, R)
     if tc:
-        _call(_typed("bl_attention_tree_tc"), ptr_q, ptr_k, ptr_v, *rest, k_cache.shape[0], H, KV, dh, page_size, window, scale, _stream().value)
+        _call(_typed("bl_attention_tree_tc"), ptr_q, ptr_k, ptr_v, *rest, k_cache.shape[0], H, KV, dh, page_size, window, scale, stream)
     else:
-        _call(_typed("bl_attention_tree"), ptr_q, ptr_k, ptr_v, _dt(q), *rest, H, KV, dh, page_size, window, scale, _stream().value)
+        _call(_typed("bl_attention_tree"), ptr_q, ptr_k, ptr_v, _dt(q), *rest, H, KV, dh, page_size, window, scale, stream)
 
 
 @functools.lru_cache(maxsize=None)
@@ -2301,7 +2312,7 @@ def accept_tree(sampled: torch.Tensor, token_ids: torch.Tensor, mask: torch.Tens
     cache rows c, c + 1, .. of `k_pages` and `v_pages` [layers, pages, kv heads, page size, head size] (contiguous layers), in place; the pages
     that hold a request's nodes must be its own."""
     T, R = _tree_step(mask, cu_q, ctx_len, block_table)
-    _fits(sampled, "sampled", torch.int32, (T,)); _fits(token_ids, "token_ids", torch.int32, (T,))
+    _list(sampled, "sampled", torch.int32, T); _list(token_ids, "token_ids", torch.int32, T)
     if k_pages.dim() != 5 or k_pages.shape != v_pages.shape:
         raise KernelError(f"k_pages, v_pages: must be [layers, pages, kv heads, page size, head size] alike, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     layers, pages, KV, page_size, dh = k_pages.shape
@@ -2310,13 +2321,13 @@ def accept_tree(sampled: torch.Tensor, token_ids: torch.Tensor, mask: torch.Tens
     least = pages * rows[0] if layers > 1 else 0
     if v_pages.dtype is not k_pages.dtype or k_stride[1:] != rows or v_stride[1:] != rows or k_stride[0] < least or v_stride[0] < least:
         raise KernelError("k_pages, v_pages: each layer must be contiguous, layers must not overlap, and the dtypes must agree")
-    _here(sampled, token_ids, mask, cu_q, ctx_len, k_pages, v_pages, block_table)
+    stream = _here(sampled, token_ids, mask, cu_q, ctx_len, k_pages, v_pages, block_table)
     device = mask.device
     counts = torch.empty(R, dtype=torch.int32, device=device)
     path, tokens = (torch.empty((R, TREE_MAX_NODES), dtype=torch.int32, device=device) for _ in range(2))
     _call(_typed("bl_accept_tree"), sampled.data_ptr(), token_ids.data_ptr(), mask.data_ptr(), cu_q.data_ptr(), ctx_len.data_ptr(),
           block_table.data_ptr(), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.element_size(), k_stride[0],
-          v_stride[0], layers, KV, page_size, dh, counts.data_ptr(), path.data_ptr(), tokens.data_ptr(), R, _stream().value)
+          v_stride[0], layers, KV, page_size, dh, counts.data_ptr(), path.data_ptr(), tokens.data_ptr(), R, stream)
     return counts, path, tokens
 
 
@@ -2324,7 +2335,10 @@ def copy_blocks(tensors, pairs) -> None:
     """t[:, target] = t[:, source] for every (source, target) of `pairs` (a list of pairs of ints) and every tensor [layers, blocks, ...] whose
     blocks are contiguous: pages, or state slots, of all layers in one launch (a launch for every 1,024 pairs). No block may be the
     target of two copies, or target and source. The pairs are part of the launch: a captured call copies the same ones again."""
-    flat = array.array("i", itertools.chain.from_iterable(pairs))
+    try:
+        flat = array.array("i", itertools.chain.from_iterable(pairs))
+    except (OverflowError, TypeError) as e:
+        raise KernelError(f"pairs: must be pairs of block numbers ({e})") from None
     if len(flat) != 2 * len(pairs):
         raise KernelError("pairs: must be pairs of block numbers")
     lists = array.array("q")
@@ -2334,8 +2348,8 @@ def copy_blocks(tensors, pairs) -> None:
         lists.extend((t.data_ptr(), layer_items * item, block_items * item, layers, blocks))
     if len(tensors) == 0 or len(flat) == 0:
         return
-    _here(*tensors)
-    _call(_typed("bl_copy_blocks"), len(tensors), lists.buffer_info()[0], flat.buffer_info()[0], len(pairs), _stream().value)
+    stream = _here(*tensors)
+    _call(_typed("bl_copy_blocks"), len(tensors), lists.buffer_info()[0], flat.buffer_info()[0], len(pairs), stream)
 
 
 @functools.lru_cache(maxsize=256)

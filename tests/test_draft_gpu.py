@@ -218,6 +218,40 @@ def test_drafts_and_forks_together(model_folders):
     eng.runner.cache.check()
 
 
+def test_a_source_that_ends_before_the_copy_is_made(model_folders):
+    """A page that a fork goes on in a copy of is given back by its source, and poisoned, before the step that copies it."""
+    from boring_llm_b200 import StepEntry
+    eng = engine(model_folders("A", "float32"), "float32", debug_poison=True)
+    run = eng.runner
+    prompt = helpers.random_tokens(256, 21, 4)
+    run.step([StepEntry("a", prompt, [])])
+    want = run.step([StepEntry("a", [7], [0])]).clone()
+    run.truncate("a", 21)
+    run.fork_request("a", "b")
+    assert run.cache.reserve("b", 1) and run.cache.has_copies         # as a scheduler reserves ahead of the step
+    run.free_request("a")
+    got = run.step([StepEntry("c", prompt[:5], []), StepEntry("b", [7], [0])])
+    assert not run.cache.has_copies and torch.equal(got, want)
+    run.cache.check()
+
+
+def test_fork_hands_on_what_ends_meanwhile(model_folders):
+    """A request that ends in the step that was launched ahead is among those that the next step returns."""
+    from boring_llm_b200.sampling.params import SamplingParams
+    eng = engine(model_folders("A", "bfloat16"), "bfloat16")
+    long, short = (eng.add_request([5, 6, 7], SamplingParams(n_predict=n, ignore_eos=True)) for n in (40, 12))
+    done = []
+    while len(short.output) < 11:
+        done += eng.step()
+    assert eng._inflight is not None and not done
+    new = eng.fork(long)
+    while not done:
+        done += eng.step()
+    assert short in done and short.finish_reason == "length"
+    eng.run_until_done()
+    assert len(new.output) == len(long.output) == 40
+
+
 @pytest.mark.parametrize("rows", [3, 40, 70, 300])
 @pytest.mark.parametrize("H,KV,dh,d,layout", [(4, 2, 64, 256, 0), (14, 2, 64, 896, 0), (4, 2, 32, 128, 1)])
 def test_cache_rows_beside_positions(rows, H, KV, dh, d, layout):

@@ -22,7 +22,7 @@ def step(**changes):
 @pytest.mark.parametrize("change,what", [
     (dict(mask=lambda t: t.int()), "mask"), (dict(mask=lambda t: t[:-1]), "q"), (dict(cu_q=lambda t: t[:-1]), "cu_q"), (dict(cu_q=lambda t: t.long()), "cu_q"),
     (dict(ctx_len=lambda t: t.float()), "ctx_len"), (dict(block_table=lambda t: t[:1]), "block_table"), (dict(block_table=lambda t: t.long()), "block_table"),
-    (dict(block_table=lambda t: t.t().contiguous().t()), "block_table"), (dict(H=3), "heads"), (dict(H=0), "heads"), (dict(H=8), "q"),
+    (dict(block_table=lambda t: t.t().contiguous().t()), "block_table"), (dict(H=3), "heads"), (dict(H=0), "heads"), (dict(k_cache=lambda t: t[:, :0], v_cache=lambda t: t[:, :0]), "heads"), (dict(H=8), "q"),
     (dict(q=lambda t: t.half()), "float32 or bfloat16"), (dict(q=lambda t: t.bfloat16()), "k_cache"), (dict(k_cache=lambda t: t[0]), "k_cache"),
     (dict(v_cache=lambda t: t[:, :, :, :8]), "v_cache"), (dict(out=lambda t: t.bfloat16()), "out"), (dict(q=lambda t: t.t().contiguous().t()), "contiguous"),
     (dict(), "CUDA")])
@@ -72,7 +72,8 @@ def test_accept_tree_refuses(change, what):
 
 @pytest.mark.parametrize("tensors,pairs,what", [
     ([torch.zeros(5)], [(0, 1)], "layers, blocks"), ([torch.zeros(2, 5, 4).transpose(1, 2)], [(0, 1)], "contiguous"),
-    ([torch.zeros(1, 5, 4).expand(3, -1, -1)], [(0, 1)], "overlap"), ([torch.zeros(2, 5, 4)], [(0, 1, 2)], "pairs"), ([torch.zeros(2, 5, 4)], [(0, 1)], "CUDA")])
+    ([torch.zeros(1, 5, 4).expand(3, -1, -1)], [(0, 1)], "overlap"), ([torch.zeros(2, 5, 4)], [(0, 1, 2)], "pairs"), ([torch.zeros(2, 5, 4)], [(0, 1 << 40)], "pairs"),
+    ([torch.zeros(2, 5, 4)], [(0, 1.5)], "pairs"), ([torch.zeros(2, 5, 4)], [(0, 1)], "CUDA")])
 def test_copy_blocks_refuses(tensors, pairs, what):
     with pytest.raises(KernelError, match=what):
         ops.copy_blocks(tensors, pairs)
