@@ -6,9 +6,12 @@
 // position is c + popcount(mask) - 1. out = sum_j softmax_j(scale q . k_j) v_j, in the online form, statistics in 32 bits:
 // m' = max(m, max s), l' = l 2^(m - m') + sum 2^(s - m'), o' = o 2^(m - m') + sum 2^(s - m') v, s in the base-2 domain.
 //
-// A block holds 64 rows (pairs of a node and a query head of a group) and walks blocks of 64 keys: S as a 64 x 64 product with 4 x 4
-// outputs a thread, P through shared memory with the keys outermost, O += P V with 4 rows x dh / 16 columns a thread. Keys of the next
-// block arrive (cp.async) under the softmax and P V, values under S. The line of work and the merge are those of attention_tree.cuh.
+// A block holds 64 rows (pairs of a node and a query head of a group) and walks blocks of 64 keys: S as a 64 x 64 product with 8 x 4
+// outputs a thread, P through shared memory with the keys outermost, O += P V with 8 rows x dh / 16 columns a thread. Values arrive
+// (cp.async) under S; the next keys under the softmax and P V where they have room beside P (head sizes up to 64), else P lies where the
+// keys were. Two blocks share an SM and hide each other's waits. Bound by shared memory's loads (12 of 16 bytes for 128 multiply-adds)
+// at large sizes (16 requests of 64 nodes at 900 to 2,000 tokens, 28 / 4 heads of 128: 780 us, 23 TFLOP/s; with 4 x 4 outputs a thread
+// 1,063), at small ones by the chain of a block's first loads and the merge (four requests of 13 nodes, 14 / 2 heads of 64: 34 us). The line of work and the merge are those of attention_tree.cuh.
 // Rows of the cache that no node of the request may see are not read: zeros stand in their place.
 #include "attention_tree.cuh"
 #include "api.h"
@@ -16,7 +19,7 @@
 
 namespace {
 
-constexpr int ROWS = 64, KEYS = 64, THREADS = 256, LDP = ROWS + 4;
+constexpr int ROWS = 64, KEYS = 64, THREADS = 128, LDP = ROWS + 4;
 
 template <typename TT>
 struct Params {
@@ -57,16 +60,18 @@ __device__ __forceinline__ void copy_rows(float* dst, int ld, const TT* src, con
 
 // NV: columns of the output a thread owns are tx * 4 + 64 * v, v < NV.
 template <typename TT, bool VEC, int NV>
-__global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kernel(const Params<TT> p) {
+__global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) attention_tree_kernel(const Params<TT> p) {
+    constexpr bool BESIDE = NV == 1;                                     // P has room beside the keys
     extern __shared__ __align__(16) float sm[];
     __shared__ long long offs[2][KEYS], q_offs[ROWS];                    // where the keys of this block and the next lie, and the rows of q
+    __shared__ unsigned long long s_seen[ROWS];                          // what each row may see
+    __shared__ int s_lo[ROWS], s_ends[32];
     __shared__ TreeShare s_share;
-    __shared__ int s_ends[32];
     const int dp = (p.dh + 3) & ~3, ld = dp + 4;
     float* qs = sm;                                                      // [ROWS][ld]
-    float* ks = qs + ROWS * ld;                                          // [KEYS][ld]
-    float* vs = ks + KEYS * ld;                                          // [KEYS][ld]
-    float* ps = vs + KEYS * ld;                                          // [KEYS][LDP]
+    float* ks = qs + ROWS * ld;                                          // [KEYS][ld], and P [KEYS][LDP] where it has no room of its own
+    float* vs = ks + (BESIDE ? KEYS * ld : max(KEYS * ld, KEYS * LDP));  // [KEYS][ld]
+    float* ps = BESIDE ? vs + KEYS * ld : ks;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     bl_pdl_wait();
     bl_pdl_trigger();
@@ -89,6 +94,7 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
         const int node0 = w.tile * p.line.npt, nodes = min(p.line.npt, rq.n - node0);
         const int* table = p.table + (size_t)w.r * p.max_pages;
         const int hi = rq.c + rq.n - 1;
+        const int lo_most = p.line.window > 0 ? max(0, rq.c + rq.n - p.line.window) : 0;     // no row's first committed key lies behind this (or behind c)
         auto place = [&](int b, int buf) {                               // where the keys of block b lie; -1: no node may see the key
             if (tid < KEYS) {
                 const int j = b * KEYS + tid;
@@ -97,33 +103,29 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
                 offs[buf][tid] = off;
             }
         };
-        // the tile's rows of q, and what each of this thread's four rows may see
         __syncthreads();                                                 // the segment before has been read
         place(w.b, 0);
-        if (tid >= KEYS && tid < KEYS + ROWS) {
+        if (tid >= KEYS) {
             const int row = tid - KEYS, node = row / p.G;
             q_offs[row] = node < nodes ? ((long long)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh : -1;
+            unsigned long long seen = 0;
+            int lo = 0x7fffffff;                                         // rows that the tile does not have see nothing
+            if (node < nodes) {
+                const unsigned long long m = p.mask[rq.begin + node0 + node];
+                const int pos = rq.c + max(__popcll(rq.n < 64 ? m & ((1ULL << rq.n) - 1) : m) - 1, 0);
+                seen = tree_mask(m, rq.n, p.line.window);
+                lo = p.line.window > 0 ? min(max(0, pos - p.line.window + 1), rq.c) : 0;
+            }
+            s_seen[row] = seen;
+            s_lo[row] = lo;
         }
         __syncthreads();
         copy_rows<TT, VEC>(qs, ld, p.q, q_offs, p.dh, dp);               // q and the first keys arrive together
         copy_rows<TT, VEC>(ks, ld, p.kc, offs[0], p.dh, dp);
-        const bool rows_here = (tid >> 5) * 8 < nodes * p.G;             // a warp has eight rows: without one it only copies
-        unsigned long long seen[4];
-        int lo[4];
+        const bool rows_here = (tid >> 5) * 16 < nodes * p.G;            // a warp has sixteen rows: without one it only copies
+        float m[8], l[8], o[8][4 * NV];
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int node = (ty * 4 + a) / p.G;
-            seen[a] = 0; lo[a] = 0x7fffffff;                             // rows that the tile does not have see nothing
-            if (node < nodes) {
-                const unsigned long long m = p.mask[rq.begin + node0 + node];
-                const int pos = rq.c + max(__popcll(rq.n < 64 ? m & ((1ULL << rq.n) - 1) : m) - 1, 0);
-                seen[a] = tree_mask(m, rq.n, p.line.window);
-                lo[a] = p.line.window > 0 ? min(max(0, pos - p.line.window + 1), rq.c) : 0;
-            }
-        }
-        float m[4], l[4], o[4][4 * NV];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
+        for (int a = 0; a < 8; ++a) {
             m[a] = -INFINITY; l[a] = 0.f;
 #pragma unroll
             for (int j = 0; j < 4 * NV; ++j) o[a][j] = 0.f;
@@ -134,120 +136,132 @@ __global__ void __launch_bounds__(THREADS, NV == 1 ? 2 : 1) attention_tree_kerne
             if (i + 1 < n_blocks) place(w.b + i + 1, buf ^ 1);
             cp_wait<1>();
             __syncthreads();                                             // keys are there
-            float s[4][4];
+            float s[8][4];
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < 8; ++a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[a][j] = 0.f;
+            if (rows_here) {
 #pragma unroll 2
-            for (int d = 0; rows_here && d < dp; d += 4) {
-                float4 qa[4], kb[4];
+                for (int d = 0; d < dp; d += 4) {
+                    float4 kb[4];
 #pragma unroll
-                for (int a = 0; a < 4; ++a) qa[a] = *reinterpret_cast<const float4*>(qs + (ty * 4 + a) * ld + d);
+                    for (int j = 0; j < 4; ++j) kb[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * ld + d);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) kb[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * ld + d);
+                    for (int a = 0; a < 8; ++a) {
+                        const float4 qa = *reinterpret_cast<const float4*>(qs + (ty * 8 + a) * ld + d);
 #pragma unroll
-                for (int a = 0; a < 4; ++a)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[a][j] = fmaf(qa[a].x, kb[j].x, s[a][j]); s[a][j] = fmaf(qa[a].y, kb[j].y, s[a][j]);
-                        s[a][j] = fmaf(qa[a].z, kb[j].z, s[a][j]); s[a][j] = fmaf(qa[a].w, kb[j].w, s[a][j]);
+                        for (int j = 0; j < 4; ++j) {
+                            s[a][j] = fmaf(qa.x, kb[j].x, s[a][j]); s[a][j] = fmaf(qa.y, kb[j].y, s[a][j]);
+                            s[a][j] = fmaf(qa.z, kb[j].z, s[a][j]); s[a][j] = fmaf(qa.w, kb[j].w, s[a][j]);
+                        }
                     }
+                }
             }
             __syncthreads();                                             // keys have been read
-            if (i + 1 < n_blocks) copy_rows<TT, VEC>(ks, ld, p.kc, offs[buf ^ 1], p.dh, dp);
+            if (BESIDE && i + 1 < n_blocks) copy_rows<TT, VEC>(ks, ld, p.kc, offs[buf ^ 1], p.dh, dp);
             else cp_commit();
             if (rows_here) {
+                if (k0 + KEYS <= rq.c && k0 >= lo_most) {                // every row sees all of these keys
 #pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                float top = -INFINITY;
+                    for (int a = 0; a < 8; ++a)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool sees = tree_bits(seen[a], rq.c, lo[a], k0 + tx + 16 * j) & 1u;
-                    s[a][j] = sees ? s[a][j] * p.scale_log2 : -INFINITY;
-                    top = fmaxf(top, s[a][j]);
+                        for (int j = 0; j < 4; ++j) s[a][j] *= p.scale_log2;
+                } else {
+#pragma unroll
+                    for (int a = 0; a < 8; ++a) {
+                        const unsigned long long seen = s_seen[ty * 8 + a];
+                        const int lo = s_lo[ty * 8 + a];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[a][j] = tree_bits(seen, rq.c, lo, k0 + tx + 16 * j) & 1u ? s[a][j] * p.scale_log2 : -INFINITY;
+                    }
                 }
 #pragma unroll
-                for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                const float m_new = fmaxf(m[a], top), m_use = m_new == -INFINITY ? 0.f : m_new;
-                const float alpha = exp2f(m[a] - m_use);
-                float sum = 0.f;
+                for (int a = 0; a < 8; ++a) {
+                    float top = fmaxf(fmaxf(s[a][0], s[a][1]), fmaxf(s[a][2], s[a][3]));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { s[a][j] = exp2f(s[a][j] - m_use); sum += s[a][j]; }
+                    for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float m_new = fmaxf(m[a], top), m_use = m_new == -INFINITY ? 0.f : m_new;
+                    const float alpha = exp2f(m[a] - m_use);
+                    float sum = 0.f;
 #pragma unroll
-                for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                l[a] = l[a] * alpha + sum;
-                m[a] = m_new;
+                    for (int j = 0; j < 4; ++j) { s[a][j] = exp2f(s[a][j] - m_use); sum += s[a][j]; }
 #pragma unroll
-                for (int j = 0; j < 4 * NV; ++j) o[a][j] *= alpha;
-            }
+                    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                    l[a] = l[a] * alpha + sum;
+                    m[a] = m_new;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(ps + (tx + 16 * j) * LDP + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+                    for (int j = 0; j < 4 * NV; ++j) o[a][j] *= alpha;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float* dst = ps + (tx + 16 * j) * LDP + ty * 8;
+                    *reinterpret_cast<float4*>(dst) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+                    *reinterpret_cast<float4*>(dst + 4) = make_float4(s[4][j], s[5][j], s[6][j], s[7][j]);
+                }
             }
             cp_wait<1>();
             __syncthreads();                                             // values and P are there
+            if (rows_here) {
 #pragma unroll 4
-            for (int j = 0; rows_here && j < KEYS; ++j) {
-                const float4 pr = *reinterpret_cast<const float4*>(ps + j * LDP + ty * 4);
+                for (int j = 0; j < KEYS; ++j) {
+                    const float4 pa = *reinterpret_cast<const float4*>(ps + j * LDP + ty * 8), pb = *reinterpret_cast<const float4*>(ps + j * LDP + ty * 8 + 4);
+                    const float pr[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
 #pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                    const int col = tx * 4 + 64 * v;
-                    if (col < dp) {
-                        const float4 x = *reinterpret_cast<const float4*>(vs + j * ld + col);
-                        const float pa[4] = {pr.x, pr.y, pr.z, pr.w};
+                    for (int v = 0; v < NV; ++v) {
+                        const int col = tx * 4 + 64 * v;
+                        if (col < dp) {
+                            const float4 x = *reinterpret_cast<const float4*>(vs + j * ld + col);
 #pragma unroll
-                        for (int a = 0; a < 4; ++a) {
-                            o[a][4 * v] = fmaf(pa[a], x.x, o[a][4 * v]); o[a][4 * v + 1] = fmaf(pa[a], x.y, o[a][4 * v + 1]);
-                            o[a][4 * v + 2] = fmaf(pa[a], x.z, o[a][4 * v + 2]); o[a][4 * v + 3] = fmaf(pa[a], x.w, o[a][4 * v + 3]);
+                            for (int a = 0; a < 8; ++a) {
+                                o[a][4 * v] = fmaf(pr[a], x.x, o[a][4 * v]); o[a][4 * v + 1] = fmaf(pr[a], x.y, o[a][4 * v + 1]);
+                                o[a][4 * v + 2] = fmaf(pr[a], x.z, o[a][4 * v + 2]); o[a][4 * v + 3] = fmaf(pr[a], x.w, o[a][4 * v + 3]);
+                            }
                         }
                     }
                 }
             }
             __syncthreads();                                             // values and P have been read
+            if (!BESIDE && i + 1 < n_blocks) copy_rows<TT, VEC>(ks, ld, p.kc, offs[buf ^ 1], p.dh, dp);
         }
         cp_wait<0>();
         const bool whole = n_blocks == rq.nb;
         const size_t slot = 2 * (size_t)blockIdx.x + (first ? 0 : 1);
         float* stats = tree_stats(p.scratch, gridDim.x, ROWS, p.dh) + slot * ROWS * 2;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int row = ty * 4 + a, node = row / p.G;
+        for (int a = 0; a < 8; ++a) {
+            const int row = ty * 8 + a, node = row / p.G;
             if (node >= nodes) continue;
             if (whole) {
                 const float inv = l[a] > 0.f ? 1.0f / l[a] : 0.f;
-                TT* dst = p.out + ((size_t)(rq.begin + node0 + node) * p.H + w.kvh * p.G + row - node * p.G) * p.dh;
+                TT* dst = p.out + q_offs[row];
 #pragma unroll
                 for (int j = 0; j < 4 * NV; ++j) {
                     const int col = tx * 4 + 64 * (j >> 2) + (j & 3);
                     if (col < p.dh) bl_store(dst + col, o[a][j] * inv);
                 }
-            } else if (tx == 0) {
-                stats[2 * row] = m[a]; stats[2 * row + 1] = l[a];
+                continue;
             }
-        }
-        if (!whole) {
+            if (tx == 0) { stats[2 * row] = m[a]; stats[2 * row + 1] = l[a]; }
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (tx * 4 + 64 * v >= dp) continue;
-#pragma unroll
-                for (int a = 0; a < 4; ++a)
-                    *tree_cols(tree_outputs(p.scratch, gridDim.x), slot, ROWS, p.dh, ty * 4 + a, tx + 16 * v) =
+            for (int v = 0; v < NV; ++v)
+                if (tx * 4 + 64 * v < dp)
+                    *tree_cols(tree_outputs(p.scratch, gridDim.x), slot, ROWS, p.dh, row, tx + 16 * v) =
                         make_float4(o[a][4 * v], o[a][4 * v + 1], o[a][4 * v + 2], o[a][4 * v + 3]);
-            }
         }
         left -= n_blocks;
         if (left > 0) tree_next_unit<KEYS>(p.line, w);
     }
 }
 
-size_t smem_bytes(int dh) { return ((size_t)(ROWS + 2 * KEYS) * (((dh + 3) & ~3) + 4) + (size_t)KEYS * LDP) * sizeof(float); }
-
-// Blocks that the device holds at once (also the number of parts that the line is cut into at most).
-int resident_blocks(int dh) {
-    const int per_sm = dh <= 64 ? 2 : 1;                                 // by registers (and 118 KB of shared memory at a head size of 128)
-    return bl_device_sms() * per_sm;
+size_t smem_bytes(int dh) {
+    const size_t row = ((dh + 3) & ~3) + 4, keys = KEYS * row, probs = (size_t)KEYS * LDP;
+    return (ROWS * row + KEYS * row + (dh <= 64 ? keys + probs : keys > probs ? keys : probs)) * sizeof(float);
 }
+
+// Blocks that the device holds at once (also the number of parts that the line is cut into at most): by registers up to a head size of 128, by
+// shared memory above.
+int resident_blocks(int dh) { return bl_device_sms() * (dh <= 128 ? 2 : 1); }
 
 template <typename TT, bool VEC, int NV>
 int launch(const Params<TT>& p, int blocks, cudaStream_t s) {
