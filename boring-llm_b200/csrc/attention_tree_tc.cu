@@ -19,10 +19,12 @@
 // Values behind the request's last row, in a page that was copied, are set to zero (0 x whatever an old request left must stay 0).
 // P is rounded to bfloat16 (half a step, 2^-8 of each weight, as the operand of a bfloat16 product must be); the sum is of the 32-bit values.
 //
-// What bounds it: at few rows the keys' way from HBM; at two full tiles the row warps' arithmetic, which waits for its own results (1.2 us
-// per 64 keys and two tiles, 2,050 cycles, of which the tensor cores work 980 and the special-function unit 670; a row's 64 scores stay in
-// registers from the load to P; key blocks of 128 in two passes over the scores took 1.7 times as long, 2^x by polynomials on the
-// FMA pipes changed nothing). 64 requests of 64 nodes, 28 / 4 heads of 128, contexts of 2,003 to 4,001: 220 us, 840 TFLOP/s.
+// What bounds it: with two full tiles the products and the hand-overs between the warps together. 64 requests of 64 nodes, 28 / 4 heads of
+// 128, contexts of 2,003 to 4,001: 217 us, 850 TFLOP/s; without the softmax's arithmetic 195, without copies 207, without both 167, of which
+// S is 50 (an MMA of N 64 reads 6 KB of shared memory in 32 cycles, more than the 4 KB there are; a key block of 128 would need
+// the tensor memory that the second pair of score buffers has) and P V 15. With one request or few, the chains at the ends: lengths, pages, first
+// copies (5 us), outputs and the merge (4 to 10 us). Tried: key blocks of 128 in two passes over the scores 1.3 times as long; one group of row warps
+// 1.6 times; 2^x by polynomials on the FMA pipes, scalar arithmetic, other orders of the exponentials: nothing.
 //
 // Every wait on an mbarrier is bounded; a block whose bound runs out records a code in a status word
 // (bl_attention_tree_tc_status), its warps leave their loops, its copies are waited for, its tensor memory is freed.
