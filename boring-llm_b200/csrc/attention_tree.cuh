@@ -60,8 +60,8 @@ struct TreeCut { int parts, first, slot, tok, nodes, kvh, items, pad; };        
 // A block's part of the line: `left` key blocks from `place` on (0: none), and what there is to merge at its beginning.
 struct TreeShare { TreePlace place; int left; TreeCut cut; };
 
-// The share of block i of `grid`, by all lanes of a warp (the same answer in each). No part has fewer than MIN blocks (of a line that has
-// them). The line is shorter than 2^31 (the host sees to it). `ends`: 32 words of shared memory.
+// The share of block i of `grid`, by all lanes of a warp (the same answer in each). No part has fewer than MIN blocks before parts
+// snap (of a line that has them). The line is shorter than 2^31 (the host sees to it). `ends`: 32 words of shared memory.
 template <int KEYS, int MIN, int SNAP>
 __device__ __forceinline__ TreeShare tree_share(const TreeLine& a, int grid, int i, int* ends) {
     constexpr unsigned ALL = 0xffffffffu;

@@ -41,6 +41,10 @@ constexpr int ROW_WARPS = 8, COPY_WARPS = 2;                             // two 
 constexpr int WARP_S = ROW_WARPS, WARP_PV = WARP_S + 1, WARP_COPY = WARP_PV + 1;
 constexpr int THREADS = 32 * (WARP_COPY + COPY_WARPS);
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
+// Of the line's parts (attention_tree.cuh): a unit of up to 7 key blocks is never cut, small units go one to a block. 64 requests of 8 nodes at
+// 30 to 100 tokens (16 / 2 heads of 128) 8.1 us, with parts of four blocks at least 15.8; 20 of 30 nodes at 100 to 400 (28 / 4) 18.5, snapped over
+// two blocks 22.4.
+constexpr int MIN = 1, SNAP = 3;
 
 template <int DH_>
 struct Shape {
@@ -200,9 +204,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     bl_pdl_wait();
-    bl_pdl_trigger();
     if (warp == 0) {
-        TreeShare s = tree_share<KEYS, 4, 2>(p.line, gridDim.x, blockIdx.x, s_ends);
+        TreeShare s = tree_share<KEYS, MIN, SNAP>(p.line, gridDim.x, blockIdx.x, s_ends);
         if (lane == 0) {
             *s_share = s;
             s.cut.items = tree_merge_items(s.cut, p.G, DH / 8);
@@ -212,6 +215,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+    bl_pdl_trigger();                                                    // the next kernel may start: this block has its tensor memory
     const uint32_t tmem = *tmem_slot;
     TreePlace w = s_share->place;
     int left = s_share->left;
@@ -605,6 +609,9 @@ int launch(const void* q, const void* k_cache, const void* v_cache, const Params
     }
     BL_CUDA(bl_launch_dependent(attention_tree_tc_kernel<S>, dim3(blocks), dim3(THREADS), (size_t)S::SMEM_BYTES, stream, mq, mk, mv, p));
     BL_CHECK_LAUNCH("bl_attention_tree_tc");
+    // the most key blocks that a unit can have: where none can be cut there is nothing to merge (one request of 8 nodes at 300: 3 us of launch)
+    const long long room = ((long long)p.max_pages * PAGE + KEYS - 1) / KEYS, seen = p.line.window > 0 ? ((long long)p.line.window + TREE_MAX_NODES + KEYS) / KEYS + 1 : room;
+    if ((room < seen ? room : seen) <= 2 * SNAP + 1) return 0;
     TreeMerge<__nv_bfloat16> mg{p.scratch, p.out, blocks, S::DH, p.H, p.G};
     BL_CUDA(bl_launch_dependent(tree_merge_kernel<UNIT_ROWS, S::DH / 8, __nv_bfloat16>, dim3(4 * blocks), dim3(32 * TREE_MERGE_WARPS), 0, stream, mg));
     BL_CHECK_LAUNCH("bl_attention_tree_tc (merge)");
