@@ -139,27 +139,34 @@ def test_step_tree_refuses(model_folders):
     run.cache.check()
 
 
+FAMILIES = ["fezopel", "kavotar", "miforax", "dapuzen", "gipinex", "zuvevik"]
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_models_with_state_refuse_drafts_but_fork(tmp_path, dtype):
-    """A fork of a request with recurrent state goes on as its source does."""
-    from boring_llm_b200 import Engine, EngineOptions, FezopelConfig
+@pytest.mark.parametrize("family", FAMILIES)
+def test_every_family_forks_and_says_whether_it_drafts(family, dtype):
+    """Recurrent state, matrix memories, latent rows, windows, chunks, one number beside a key, a request's last token: a fork goes on as
+    its source does. Drafts are refused where a mixer keeps state or attends in a way of its own."""
+    import importlib
+    import boring_llm_b200 as b
     from boring_llm_b200.sampling.params import SamplingParams
-    import test_fezopel_gpu as fez
-    cfg = FezopelConfig.from_dict(next(iter(fez.SHAPES.values())))
-    opts = dict(dtype=dtype, ctx_size=128, max_num_seqs=4, max_tokens=1024)
-    with pytest.raises(ValueError, match="draft_tokens"):
-        Engine.from_random(cfg, 0, EngineOptions(draft_tokens=4, **opts), std=0.2)
-    eng = Engine.from_random(cfg, 0, EngineOptions(**opts), std=0.2)
-    req = eng.add_request([3, 9, 4, 7, 1, 2, 8] * 3, SamplingParams(n_predict=40, ignore_eos=True))
-    while len(req.output) < 9:
-        eng.step()
-    new = eng.fork(req)
-    assert new.output == req.output
-    eng.run_until_done()
-    if dtype == "float32":
-        assert new.output == req.output and len(new.output) == 40
-    eng.runner.cache.check()
-    assert eng.stats()["live_requests"] == 0
+    shapes = importlib.import_module(f"test_{family}_gpu").SHAPES
+    for raw in shapes.values():
+        cfg = getattr(b, f"{family.capitalize()}Config").from_dict(raw)
+        opts = dict(dtype=dtype, ctx_size=128, max_num_seqs=4, max_tokens=1024, device="cuda:0")
+        with pytest.raises(ValueError, match="draft_tokens"):
+            b.Engine.from_random(cfg, 0, b.EngineOptions(draft_tokens=4, **opts), std=0.2)
+        eng = b.Engine.from_random(cfg, 0, b.EngineOptions(debug_poison=True, **opts), std=0.2)
+        req = eng.add_request([3, 9, 4, 7, 1, 2, 8] * 5, SamplingParams(n_predict=60, ignore_eos=True))
+        while len(req.output) < 9:
+            eng.step()
+        new = eng.fork(req)
+        assert new.output == req.output
+        eng.run_until_done()
+        if dtype == "float32":
+            assert new.output == req.output and len(new.output) == 60
+        eng.runner.cache.check()
+        assert eng.stats()["live_requests"] == 0
 
 
 @pytest.mark.parametrize("name", ["A", "C"])

@@ -56,6 +56,21 @@ def test_attention_tree_cut_keys(requests, committed, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_tree_many_requests(dtype):
+    """More requests than lanes, several a lane, some of them without nodes; rows behind the last request stay as they were."""
+    counts = [(r * 7) % 5 for r in range(333)]
+    s = TreeStep(counts, [(r * 13) % 90 for r in range(333)], 4, 2, 64, 16, dtype, 13, device=DEV)
+    T = sum(counts)
+    s.q = torch.cat([s.q, torch.full((9, 256), float("nan"), dtype=dtype, device=DEV)])
+    s.mask = torch.cat([s.mask, torch.ones(9, dtype=torch.int64, device=DEV)])
+    out = torch.full_like(s.q, 7.0)
+    s.run(out=out)
+    assert (out[T:] == 7.0).all()
+    s.q, s.mask = s.q[:T], s.mask[:T]
+    s.check(out[:T], probabilities_bf16=dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dh", [64, 40])
 def test_attention_tree_any_mask(dh, dtype):
     """Masks that are no trees: rows that see nothing (with and without committed rows), later nodes, nodes that are not there."""
