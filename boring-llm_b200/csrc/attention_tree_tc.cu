@@ -1,6 +1,6 @@
 // Attention of the nodes of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores: bfloat16, head sizes 64
 // and 128, pages of 16. Formula, masks and positions are those of attention_tree.cu, the line of work that the blocks share out and the merge
-// of units that are cut those of attention_tree.cuh (128 rows, 128 keys).
+// of units that are cut those of attention_tree.cuh (units of 256 rows, blocks of 64 keys).
 //
 // One block per SM walks its part of the line, segment by segment (a segment: some key blocks of one unit, which is one or two tiles of 128
 // rows), through one pipeline that does not drain between segments:

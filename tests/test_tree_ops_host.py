@@ -70,6 +70,12 @@ def test_accept_tree_refuses(change, what):
         ops.accept_tree(**accept_args(**change))
 
 
+def test_accept_tree_refuses_keys_that_are_the_values():
+    args = accept_args()
+    with pytest.raises(KernelError, match="two tensors"):
+        ops.accept_tree(**dict(args, v_pages=args["k_pages"]))
+
+
 @pytest.mark.parametrize("tensors,pairs,what", [
     ([torch.zeros(5)], [(0, 1)], "layers, blocks"), ([torch.zeros(2, 5, 4).transpose(1, 2)], [(0, 1)], "contiguous"),
     ([torch.zeros(1, 5, 4).expand(3, -1, -1)], [(0, 1)], "overlap"), ([torch.zeros(2, 5, 4)], [(0, 1, 2)], "pairs"), ([torch.zeros(2, 5, 4)], [(0, 1 << 40)], "pairs"),
