@@ -87,6 +87,9 @@ __global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) attention_tree_kerne
     TreePlace w = s_share.place;
     int left = s_share.left;
     const long long page_stride = (long long)p.line.KV * p.page_size * p.dh;
+    int cols[NV];                                                        // columns past the head size take the last ones again: no branch, not stored
+#pragma unroll
+    for (int v = 0; v < NV; ++v) cols[v] = min(tx * 4 + 64 * v, dp - 4);
 
     for (bool first = true; left > 0; first = false) {
         const TreeRequest& rq = w.q;
@@ -209,14 +212,11 @@ __global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) attention_tree_kerne
                     const float pr[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
 #pragma unroll
                     for (int v = 0; v < NV; ++v) {
-                        const int col = tx * 4 + 64 * v;
-                        if (col < dp) {
-                            const float4 x = *reinterpret_cast<const float4*>(vs + j * ld + col);
+                        const float4 x = *reinterpret_cast<const float4*>(vs + j * ld + cols[v]);
 #pragma unroll
-                            for (int a = 0; a < 8; ++a) {
-                                o[a][4 * v] = fmaf(pr[a], x.x, o[a][4 * v]); o[a][4 * v + 1] = fmaf(pr[a], x.y, o[a][4 * v + 1]);
-                                o[a][4 * v + 2] = fmaf(pr[a], x.z, o[a][4 * v + 2]); o[a][4 * v + 3] = fmaf(pr[a], x.w, o[a][4 * v + 3]);
-                            }
+                        for (int a = 0; a < 8; ++a) {
+                            o[a][4 * v] = fmaf(pr[a], x.x, o[a][4 * v]); o[a][4 * v + 1] = fmaf(pr[a], x.y, o[a][4 * v + 1]);
+                            o[a][4 * v + 2] = fmaf(pr[a], x.z, o[a][4 * v + 2]); o[a][4 * v + 3] = fmaf(pr[a], x.w, o[a][4 * v + 3]);
                         }
                     }
                 }
