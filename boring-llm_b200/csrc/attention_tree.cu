@@ -9,9 +9,12 @@
 // A block holds 64 rows (pairs of a node and a query head of a group) and walks blocks of 64 keys: S as a 64 x 64 product with 8 x 4
 // outputs a thread, P through shared memory with the keys outermost, O += P V with 8 rows x dh / 16 columns a thread. Values arrive
 // (cp.async) under S; the next keys under the softmax and P V where they have room beside P (head sizes up to 64), else P lies where the
-// keys were. Two blocks share an SM and hide each other's waits. Bound by shared memory's loads (12 of 16 bytes for 128 multiply-adds)
-// at large sizes (16 requests of 64 nodes at 900 to 2,000 tokens, 28 / 4 heads of 128: 780 us, 23 TFLOP/s; with 4 x 4 outputs a thread
-// 1,063), at small ones by the chain of a block's first loads and the merge (four requests of 13 nodes, 14 / 2 heads of 64: 34 us). The line of work and the merge are those of attention_tree.cuh.
+// keys were. Two blocks share an SM and hide each other's waits. Bound by the loads from shared memory together with the multiply-adds at large
+// sizes (12 loads, two wavefronts each, for 128; 16 requests of 64 nodes at 900 to 2,000 tokens, 28 / 4 heads of 128: 659 us, 27 TFLOP/s;
+// with 4 x 4 outputs a thread 1,063, with a branch for the columns past the head size in P V 780). At small sizes a chain: lengths and
+// pages 3 us, first loads 2, S 3.5, softmax 1.5, P V 3.3, outputs 1, merge 8 (four requests of 13 nodes, 14 / 2 heads of 64: 30.5 us). Tried
+// without gain: two multiply-adds to an instruction (f32x2); parts counted in halves of key blocks. The line of work and the merge are those of
+// attention_tree.cuh.
 // Rows of the cache that no node of the request may see are not read: zeros stand in their place.
 #include "attention_tree.cuh"
 #include "api.h"
