@@ -18,7 +18,6 @@
 // Rows of the cache that no node of the request may see are not read: zeros stand in their place.
 #include "attention_tree.cuh"
 #include "api.h"
-#include <atomic>
 
 namespace {
 
@@ -268,12 +267,9 @@ int resident_blocks(int dh) { return bl_device_sms() * (dh <= 128 ? 2 : 1); }
 
 template <typename TT, bool VEC, int NV>
 int launch(const Params<TT>& p, int blocks, cudaStream_t s) {
-    static std::atomic<bool> configured{false};
+    static std::atomic<unsigned long long> allowed{0};
     const size_t smem = smem_bytes(p.dh);
-    if (!configured) {
-        BL_CUDA(cudaFuncSetAttribute(attention_tree_kernel<TT, VEC, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(64 * NV)));
-        configured = true;
-    }
+    BL_CUDA(tree_allow_smem((const void*)attention_tree_kernel<TT, VEC, NV>, (int)smem_bytes(64 * NV), allowed));
     BL_CUDA(bl_launch_dependent(attention_tree_kernel<TT, VEC, NV>, dim3(blocks), dim3(THREADS), smem, s, p));
     BL_CHECK_LAUNCH("bl_attention_tree");
     TreeMerge<TT> mg{p.scratch, p.out, blocks, p.dh, p.H, p.G};

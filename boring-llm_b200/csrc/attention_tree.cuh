@@ -11,6 +11,7 @@
 // order of the line.
 #pragma once
 #include "common.cuh"
+#include <atomic>
 
 constexpr int TREE_MAX_NODES = 64;     // a node's view of its request's nodes is one 64-bit mask
 
@@ -169,6 +170,18 @@ __device__ __forceinline__ float* tree_stats(float* scratch, int blocks, int row
 // Columns 4 c4 .. of a row
 __device__ __forceinline__ float4* tree_cols(float* outputs, size_t slot, int rows, int dh, int row, int c4) {
     return reinterpret_cast<float4*>(outputs + slot * tree_slot(rows, dh)) + (size_t)c4 * rows + row;
+}
+
+// Lets a kernel have `bytes` of shared memory on the current device (the limit is the device's, once on each: `done` has their bits).
+inline cudaError_t tree_allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ULL << (dev & 63);
+    if (done.load() & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
 }
 
 template <typename TT>

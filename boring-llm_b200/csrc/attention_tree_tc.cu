@@ -602,11 +602,8 @@ int launch(const void* q, const void* k_cache, const void* v_cache, const Params
     const cuuint64_t dims[4] = {64, 8, (cuuint64_t)S::ATOMS, (cuuint64_t)p.no_group}, strides[3] = {DH * 2, 128, 8 * DH * 2};
     const cuuint32_t box[4] = {64, 8, (cuuint32_t)S::ATOMS, 2};
     if (make_map(&mq, q, 3, q_dims, q_strides, q_box) || make_map(&mk, k_cache, 4, dims, strides, box) || make_map(&mv, v_cache, 4, dims, strides, box)) return 1;
-    static std::atomic<bool> configured{false};
-    if (!configured) {
-        BL_CUDA(cudaFuncSetAttribute(attention_tree_tc_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES));
-        configured = true;
-    }
+    static std::atomic<unsigned long long> allowed{0};
+    BL_CUDA(tree_allow_smem((const void*)attention_tree_tc_kernel<S>, S::SMEM_BYTES, allowed));
     BL_CUDA(bl_launch_dependent(attention_tree_tc_kernel<S>, dim3(blocks), dim3(THREADS), (size_t)S::SMEM_BYTES, stream, mq, mk, mv, p));
     BL_CHECK_LAUNCH("bl_attention_tree_tc");
     // the most key blocks that a unit can have: where none can be cut there is nothing to merge (one request of 8 nodes at 300: 3 us of launch)
