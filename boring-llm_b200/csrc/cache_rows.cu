@@ -11,7 +11,7 @@ namespace {
 // Node i of a request (at most 64) holds a token; mask[i] has the bits of its ancestors and its own; sampled[i] is the token that the
 // model gives behind node i. Node 0 (a token that is certain) is accepted; any other node i is when its token is the one sampled
 // behind its parent, the highest ancestor bit, and all nodes on its way are. No walk is needed: the nodes that agree
-// with their parents are one 64-bit word A (a ballot), and node i is accepted when mask[i] & ~A = 0. The deepest accepted node
+// with their parents are one 64-bit word A (a ballot), and node i is accepted when it is one of them and mask[i] & ~A = 0. The deepest accepted node
 // (the lowest of several) ends the path. Node j of the path moves from cache row c + path[j] to c + j, in every layer: since path[j] >= j a
 // thread that takes its 16 bytes of a few rows before it writes them, in ascending order, overwrites nothing that it still needs, and no
 // two threads share a byte.
@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(THREADS) accept_tree_kernel(const Accept p) {
         const unsigned long long A = ((unsigned long long)agree[1] << 32) | agree[0];
         int key = 0;                                                     // depth, then the lower node
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (m[h] != 0 && (m[h] & ~A) == 0) key = max(key, __popcll(m[h]) * NODES + NODES - 1 - (tid + 32 * h));
+        for (int h = 0; h < 2; ++h)                                      // (a mask without its node's own bit has no node that agrees)
+            if ((agree[h] >> tid & 1) && (m[h] & ~A) == 0) key = max(key, __popcll(m[h]) * NODES + NODES - 1 - (tid + 32 * h));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
         const unsigned long long way = key ? s_mask[NODES - 1 - (key & (NODES - 1))] : 0;
