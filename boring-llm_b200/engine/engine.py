@@ -101,7 +101,6 @@ class Engine:
                 if said is None:
                     sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
                     return self._finish_step(sched, sampled, t0)
-                self.runner.check_kernels()
                 self.stats_time["engine_steps"] += 1
                 self.stats_time["step_seconds"] += time.perf_counter() - t0
                 return self.scheduler.apply_drafted(sched, said)

@@ -250,10 +250,10 @@ class _TreeBatch:
         from ..kernels import ops
         torch.cuda.synchronize()
         before = ops.launch_count
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph, pool=runner._step_graph_pool()):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=runner._step_graph_pool()):
             self.run(runner)
-        self.kernels = ops.launch_count - before
+        self.graph, self.kernels = graph, ops.launch_count - before
 
     def read(self, R: int):
         """(counts [R], tokens [R, 64]) on the host, once the step has run."""
@@ -823,7 +823,8 @@ class ModelRunner:
         from node 0 whose tokens are the sampled ones. Returns, per entry, the tokens sampled along that path (one more than
         there were drafted tokens on it): the same that one step after the other would have sampled, from the same random numbers.
         All but the last are in the cache then, behind the token of node 0. `rows` holds one (params, generator, history)
-        per entry; a repeat penalty is refused (StepError), as is a model that keeps more of a request than pages."""
+        per entry; a repeat penalty is refused (StepError), as is a model that keeps more of a request than pages. A step that fails, also
+        when a kernel has given up on a bounded wait (looked at here, before anything is kept), leaves requests and generators as they were."""
         if not self.takes_trees:
             raise StepError("this model does not run trees of drafted tokens: a mixer keeps state, or attends in a way of its own")
         if not entries or len(rows) != len(entries):
@@ -861,37 +862,46 @@ class ModelRunner:
         self.storage.copy_pages()
         R, T = len(entries), sum(len(e.tokens) for e in entries)
         shape = None
-        if self._graphs_usable(entries) and T <= TREE_GRAPH_MAX_NODES:
-            # padded to a shape that other steps share: each padding node a request of its own on the spare page, then empty requests
-            T_b = -(-T // 16) * 16 if T <= 64 else -(-T // 64) * 64
-            shape = (T_b, -(-(R + T_b - T) // 8) * 8)
-            batch = self._tree_graphs.pop(shape, None)
-            if batch is None and len(self._tree_graphs) >= STEP_GRAPH_CACHE:
-                del self._tree_graphs[next(iter(self._tree_graphs))]
-            batch = self._tree_graphs[shape] = batch if batch is not None else _TreeBatch(self, *shape)   # most recently used last
-            batch.uses += 1
-        else:
-            batch = _TreeBatch(self, T, R)
-        draws = batch.fill(self, entries, rows, masks)
-        batch.dev.copy_(batch.host, non_blocking=True)
-        self.last_h2d_bytes = 4 * batch.host.numel()
-        self.last_step_graph_kernels = 0
-        if batch.graph is not None:
-            batch.graph.replay()
-            self.last_step_graph_kernels = batch.kernels
-            self.graph_steps += 1
-        else:
-            batch.run(self)
-        self._waits_unchecked = self._waits_unchecked or self.fast
-        counts, tokens = batch.read(R)
-        self.last_d2h_bytes = 4 * R * (1 + MAX_NODES)
-        if shape is not None and batch.graph is None and 0 < self.options.step_graph_after <= batch.uses:
-            batch.capture(self)                          # (this step has run; the capture itself runs nothing)
+        try:
+            if self._graphs_usable(entries) and T <= TREE_GRAPH_MAX_NODES:
+                # padded to a shape that other steps share: each padding node a request of its own on the spare page, then empty requests
+                T_b = -(-T // 16) * 16 if T <= 64 else -(-T // 64) * 64
+                shape = (T_b, -(-(R + T_b - T) // 8) * 8)
+                batch = self._tree_graphs.pop(shape, None)
+                if batch is None and len(self._tree_graphs) >= STEP_GRAPH_CACHE:
+                    del self._tree_graphs[next(iter(self._tree_graphs))]
+                batch = self._tree_graphs[shape] = batch if batch is not None else _TreeBatch(self, *shape)   # most recently used last
+                batch.uses += 1
+            else:
+                batch = _TreeBatch(self, T, R)
+            draws = batch.fill(self, entries, rows, masks)
+            batch.dev.copy_(batch.host, non_blocking=True)
+            self.last_h2d_bytes = 4 * batch.host.numel()
+            self.last_step_graph_kernels = 0
+            if batch.graph is not None:
+                batch.graph.replay()
+                self.last_step_graph_kernels = batch.kernels
+                self.graph_steps += 1
+            else:
+                batch.run(self)
+            self._waits_unchecked = self._waits_unchecked or self.fast
+            counts, tokens = batch.read(R)
+            self.last_d2h_bytes = 4 * R * (1 + MAX_NODES)
+            self.check_kernels()
+            for e, n in zip(entries, counts):
+                if n < 1:
+                    raise StepError(f"request {e.request_id!r}: the step accepted no node (node 0 is always accepted)")
+            if shape is not None and batch.graph is None and 0 < self.options.step_graph_after <= batch.uses:
+                batch.capture(self)                      # (this step has run; the capture itself runs nothing)
+        except BaseException:
+            # nothing of a step that failed is kept: no token is committed, no generator has moved, and the nodes' pages go back (what
+            # they hold lies behind the requests' tokens)
+            for e in entries:
+                self.cache.truncate(e.request_id, self.cache.get(e.request_id).num_tokens)
+            raise
         said = []
         for r, (e, (params, rng, _)) in enumerate(zip(entries, rows)):
             n = int(counts[r])
-            if n < 1:
-                raise StepError(f"request {e.request_id!r}: the step accepted no node (node 0 is always accepted)")
             self.cache.commit(e.request_id, n)
             if params.temperature > 0:
                 rng.state = draws[r][n - 1]

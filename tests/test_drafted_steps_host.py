@@ -1,0 +1,85 @@
+"""What the host does around a step of drafted trees: what it keeps, gives back, pads, and what a failure leaves behind."""
+import pytest
+import torch
+
+import drafted_steps as steps
+from boring_llm_b200 import EngineOptions, StepEntry, TreeEntry
+from boring_llm_b200.cache import CacheManager, PagedKVSpec
+from boring_llm_b200.engine import OutOfPages, StepError
+from boring_llm_b200.engine.scheduler import FINISHED, RUNNING, AdmissionError, Scheduler
+from boring_llm_b200.kernels import KernelError, ops
+from boring_llm_b200.sampling.params import SamplingParams, XorShift64
+
+FULL, WIN = PagedKVSpec(1, 4, 0), PagedKVSpec(1, 4, 20)
+
+
+def chain(rid, n, first=1):
+    return TreeEntry(rid, [first] * n, [-1] + list(range(n - 1)))
+
+
+def row(**kw):
+    params = SamplingParams(**kw)
+    return params, XorShift64(params.seed), None
+
+
+def gave_up():
+    raise KernelError("a block gave up on a bounded wait (made up by the test)")
+
+
+# ---- a step that fails ---------------------------------------------------------------------------------------------------
+
+
+def test_a_failed_tree_step_changes_nothing(monkeypatch):
+    """A wait that ran out is seen before tokens are committed and generators advance: cache, pages and random numbers are as they were."""
+    steps.host(monkeypatch, steps.whole_chains)
+    run = steps.runner()
+    rows = []
+    for i, n in enumerate((20, 16)):
+        steps.put(run, i, n)
+        rows.append(row(temperature=1.0, seed=i))
+    states, free = [r[1].state for r in rows], run.cache.free_pages()
+    run.check_kernels = gave_up
+    for _ in range(2):
+        with pytest.raises(KernelError):
+            run.step_tree([chain(0, 30), chain(1, 5)], rows)
+        assert [run.cache.get(i).num_tokens for i in (0, 1)] == [20, 16] and run.cache.free_pages() == free
+        assert [r[1].state for r in rows] == states and run.accepted == run.drafted == run.steps == 0
+        run.cache.check()
+    run.check_kernels = lambda: None
+    assert run.step_tree([chain(0, 30), chain(1, 5)], rows) == [[7] * 30, [7] * 5]
+    assert [run.cache.get(i).num_tokens for i in (0, 1)] == [50, 21]
+
+
+def test_a_tree_step_that_accepts_nothing_changes_nothing(monkeypatch):
+    """No request's tokens are committed when the answer of another one is impossible."""
+    def says(batch, R):
+        counts, tokens = steps.only_node_0(batch, R)
+        counts[1] = 0
+        return counts, tokens
+    steps.host(monkeypatch, says)
+    run = steps.runner()
+    rows = [row(temperature=1.0, seed=i) for i in range(3)]
+    for i in range(3):
+        steps.put(run, i, 16)
+    states, free = [r[1].state for r in rows], run.cache.free_pages()
+    with pytest.raises(StepError):
+        run.step_tree([chain(i, 4) for i in range(3)], rows)
+    assert [run.cache.get(i).num_tokens for i in range(3)] == [16] * 3 and run.cache.free_pages() == free
+    assert [r[1].state for r in rows] == states and run.accepted == run.drafted == 0
+    run.cache.check()
+
+
+def test_the_engine_goes_on_after_a_failed_drafted_step(monkeypatch):
+    """The requests' records and the cache agree after the error, and the next step feeds the same token at the same place."""
+    steps.host(monkeypatch, steps.whole_chains)
+    eng = steps.engine(monkeypatch)
+    req = steps.hold(eng, [1, 2, 3, 1, 2, 3], SamplingParams(n_predict=40, ignore_eos=True))
+    eng.runner.check_kernels = gave_up
+    with pytest.raises(KernelError):
+        eng.step()
+    eng.runner.cache.check()
+    assert req.state == RUNNING and req.output == [1]
+    assert eng.runner.cache.get(req.request_id).num_tokens == req.num_computed == 6
+    eng.runner.check_kernels = lambda: None
+    assert eng.step() == []
+    assert eng.runner.cache.get(req.request_id).num_tokens == req.num_computed == 6 + len(req.output) - 1 > 6
