@@ -96,18 +96,19 @@ class Engine:
                 return []
             # the third item is the request itself: its token history is only put together if a penalty asks for it
             rows = [(r.params, r.rng, r) for r, s in zip(sched.requests, sched.samples) if s]
-            if self.options.draft_tokens:
-                said = self._drafted_step(sched, rows)
-                if said is None:
-                    sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
-                    return self._finish_step(sched, sampled, t0)
+            said = self._drafted_step(sched, rows) if self.options.draft_tokens else None
+            if said is not None:
                 self.stats_time["engine_steps"] += 1
                 self.stats_time["step_seconds"] += time.perf_counter() - t0
                 return self.scheduler.apply_drafted(sched, said)
-            pending = self.runner.launch_decode(sched.entries, rows) if self.options.lookahead else None
+            pending = self.runner.launch_decode(sched.entries, rows) if self.options.lookahead and not self.options.draft_tokens else None
             if pending is None:
-                sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
-                return self._finish_step(sched, sampled, t0)
+                try:
+                    sampled = self.runner.step_and_sample(sched.entries, rows, self.sampler)
+                    return self._finish_step(sched, sampled, t0)
+                except BaseException:
+                    self._abort_rows(r for r in sched.requests if self._is_ahead(r))
+                    raise
             self._inflight = (sched, pending)
         sched, pending = self._inflight
         ahead = self.scheduler.lookahead(sched)
@@ -161,6 +162,11 @@ class Engine:
         self.runner.storage.copy_slot(source.slot, self.runner.cache.get(new.request_id).slot)
         return new
 
+    def _is_ahead(self, request) -> bool:
+        """Whether the cache holds tokens of the request that its record does not know of: of a step that failed once they were committed."""
+        held = self.runner.cache.find(request.request_id)
+        return held is not None and held.num_tokens != request.num_computed
+
     def _abort_rows(self, requests) -> None:
         seen = set()
         for r in requests:
@@ -175,7 +181,11 @@ class Engine:
         if self._inflight is None:
             return []
         (sched, pending), self._inflight = self._inflight, None
-        return self._finish_step(sched, self.runner.collect_decode(pending), time.perf_counter())
+        try:
+            return self._finish_step(sched, self.runner.collect_decode(pending), time.perf_counter())
+        except BaseException:
+            self._abort_rows(sched.requests)              # its tokens are committed: as in `step`
+            raise
 
     def _finish_step(self, sched, sampled, t0) -> List[Request]:
         self.runner.check_kernels()

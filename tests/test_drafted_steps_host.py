@@ -83,3 +83,48 @@ def test_the_engine_goes_on_after_a_failed_drafted_step(monkeypatch):
     eng.runner.check_kernels = lambda: None
     assert eng.step() == []
     assert eng.runner.cache.get(req.request_id).num_tokens == req.num_computed == 6 + len(req.output) - 1 > 6
+
+
+@pytest.mark.parametrize("draft_tokens", [0, 8])
+def test_a_failed_step_that_has_committed_ends_its_requests(monkeypatch, draft_tokens):
+    """A step without drafts has committed its tokens by the time that its kernels are checked: its requests end with an error, the others stay."""
+    steps.host(monkeypatch)
+    eng = steps.engine(monkeypatch, draft_tokens=draft_tokens, lookahead=False)
+
+    def step_and_sample(entries, rows, sampler):
+        for e in entries:
+            eng.runner.cache.commit(e.request_id, len(e.tokens))
+        return [5] * len(rows)
+    eng.runner.step_and_sample = step_and_sample
+    req = steps.hold(eng, [1, 2, 3, 4], SamplingParams(n_predict=40, ignore_eos=True, repeat_penalty=1.1))
+    eng.runner.check_kernels = gave_up
+    with pytest.raises(KernelError):
+        eng.step()
+    eng.runner.cache.check()
+    assert req.state == FINISHED and req.finish_reason == "error" and not eng.scheduler.has_work()
+    assert eng.runner.cache.live_requests() == []
+    # one that fails before anything is committed leaves its requests as they were
+    eng.runner.check_kernels = lambda: None
+    req = steps.hold(eng, [1, 2, 3, 4], SamplingParams(n_predict=40, ignore_eos=True, repeat_penalty=1.1))
+    eng.runner.step_and_sample = lambda *a: gave_up()
+    with pytest.raises(KernelError):
+        eng.step()
+    assert req.state == RUNNING and req.num_computed == eng.runner.cache.get(req.request_id).num_tokens == 4
+    eng.runner.step_and_sample = step_and_sample
+    assert eng.step() == [] and req.output[-1] == 5
+
+
+def test_a_failed_drain_ends_the_requests_of_the_step_ahead(monkeypatch):
+    """`drain` reads a step whose tokens are committed: when that fails its requests end, as they do inside `step`."""
+    steps.host(monkeypatch)
+    eng = steps.engine(monkeypatch, draft_tokens=0)
+    req = steps.hold(eng, [1, 2, 3, 4], SamplingParams(n_predict=40, ignore_eos=True))
+    sched = eng.scheduler.schedule()
+    eng.runner.cache.commit(req.request_id, 1)                    # as launching the step does
+    eng._inflight = (sched, None)
+    eng.runner.collect_decode = lambda pending: [5]
+    eng.runner.check_kernels = gave_up
+    with pytest.raises(KernelError):
+        eng.fork(req)
+    eng.runner.cache.check()
+    assert req.finish_reason == "error" and eng.runner.cache.live_requests() == [] and eng._inflight is None
