@@ -357,6 +357,10 @@ class CacheManager:
                     g.pool.give_back(p, request_id)
         rc.num_tokens = n_keep
 
+    def release_ahead(self, request_id) -> None:
+        """Gives back the pages that were reserved for tokens which have not come: what lies behind the last token's page."""
+        self.truncate(request_id, self.get(request_id).num_tokens)
+
     def free(self, request_id) -> None:
         """The request ends (or is preempted): every page and its slot go back."""
         rc = self.get(request_id)

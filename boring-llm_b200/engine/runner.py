@@ -897,12 +897,13 @@ class ModelRunner:
             # nothing of a step that failed is kept: no token is committed, no generator has moved, and the nodes' pages go back (what
             # they hold lies behind the requests' tokens)
             for e in entries:
-                self.cache.truncate(e.request_id, self.cache.get(e.request_id).num_tokens)
+                self.cache.release_ahead(e.request_id)
             raise
         said = []
         for r, (e, (params, rng, _)) in enumerate(zip(entries, rows)):
             n = int(counts[r])
             self.cache.commit(e.request_id, n)
+            self.cache.release_ahead(e.request_id)        # the pages of rejected nodes
             if params.temperature > 0:
                 rng.state = draws[r][n - 1]
             said.append([int(t) for t in tokens[r, :n]])

@@ -128,3 +128,34 @@ def test_a_failed_drain_ends_the_requests_of_the_step_ahead(monkeypatch):
         eng.fork(req)
     eng.runner.cache.check()
     assert req.finish_reason == "error" and eng.runner.cache.live_requests() == [] and eng._inflight is None
+
+
+# ---- pages ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("specs", [[FULL], [FULL, WIN]])
+def test_pages_of_rejected_nodes_go_back(monkeypatch, specs):
+    """A rejected tree leaves as many pages free as a step of one token."""
+    steps.host(monkeypatch)
+    run, plain = steps.runner(specs, max_tokens=640), CacheManager(specs, 16, 640, 16)
+    for i, n in enumerate((16, 31, 32, 5)):
+        steps.put(run, i, n)
+        plain.add_request(i)
+        assert plain.reserve(i, n)
+        plain.commit(i, n)
+    for _ in range(20):
+        run.step_tree([chain(i, 40 + i) for i in range(4)], [row() for _ in range(4)])
+        for i in range(4):
+            assert plain.reserve(i, 1)
+            plain.commit(i, 1)
+        assert run.cache.free_pages() == plain.free_pages()
+        run.cache.check()
+
+
+def test_pages_of_accepted_nodes_stay(monkeypatch):
+    steps.host(monkeypatch, steps.whole_chains)
+    run = steps.runner()
+    steps.put(run, 0, 20)
+    run.step_tree([chain(0, 30)], [row()])
+    assert run.cache.get(0).num_tokens == 50 and len(run.cache.get(0).tables[0]) == 4
+    run.cache.check()
