@@ -248,6 +248,23 @@ class CacheManager:
         """Pages that `n_new` more tokens take from each group's pool (the copy of a shared page among them)."""
         return self._pages_needed(self.get(request_id), n_new)
 
+    def pages_needed_together(self, wants: Sequence[Tuple[object, int]]) -> List[int]:
+        """Pages that a step takes from each group's pool: (request, new tokens) pairs, reserved one behind the other. Of a shared page's
+        owners the last one writes in place if all of them write."""
+        need = [0] * len(self.paged_groups)
+        writers: Dict[Tuple[int, int], int] = {}              # (group, shared page) -> requests that are about to write to it
+        for request_id, n_new in wants:
+            rc = self.get(request_id)
+            for gi, (n, group, table) in enumerate(zip(self._pages_needed(rc, n_new), self.paged_groups, rc.tables)):
+                need[gi] += n
+                if rc.forked and self._writes_shared(rc, group, table):
+                    at = gi, table[rc.num_tokens // self.page_size]
+                    writers[at] = writers.get(at, 0) + 1
+        for (gi, page), n in writers.items():
+            if n == len(self.paged_groups[gi].pool.owners_of(page)):
+                need[gi] -= 1
+        return need
+
     def can_reserve(self, request_id, n_new: int) -> bool:
         rc = self.get(request_id)
         need = self._pages_needed(rc, n_new)

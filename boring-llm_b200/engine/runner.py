@@ -629,15 +629,17 @@ class ModelRunner:
         if len(new_ids) > free_slots:
             raise StepError(f"{len(new_ids)} new requests but only {free_slots} free request slots")
         # all-or-nothing reservation across the whole batch
-        need = [0] * len(self.cache.paged_groups)
+        new_pages, held_wants = 0, []
         for e in entries:
-            held = self.cache.get(e.request_id) if e.request_id in self.cache else None
+            held = self.cache.find(e.request_id)
             n_have = held.num_tokens if held else 0
             if n_have + len(e.tokens) > self.options.ctx_size:
                 raise StepError(f"request {e.request_id!r}: {n_have + len(e.tokens)} tokens exceed the context size {self.options.ctx_size}")
-            each = self.cache.pages_needed(e.request_id, len(e.tokens)) if held else [-(-len(e.tokens) // page)] * len(need)
-            for gi in range(len(need)):
-                need[gi] += each[gi]
+            if held:
+                held_wants.append((e.request_id, len(e.tokens)))
+            else:
+                new_pages += -(-len(e.tokens) // page)
+        need = [n + new_pages for n in self.cache.pages_needed_together(held_wants)]
         free = self.cache.free_pages()
         if any(n > f for n, f in zip(need, free)):
             raise OutOfPages(f"the step needs {need} pages per group, {free} are free")
@@ -850,7 +852,7 @@ class ModelRunner:
                 raise StepError(f"request {e.request_id!r} is not live")
             if rc.num_tokens + len(e.tokens) > self.options.ctx_size:
                 raise StepError(f"request {e.request_id!r}: {rc.num_tokens + len(e.tokens)} tokens exceed the context size {self.options.ctx_size}")
-        need = [sum(n) for n in zip(*(self.cache.pages_needed(e.request_id, len(e.tokens)) for e in entries))]
+        need = self.cache.pages_needed_together([(e.request_id, len(e.tokens)) for e in entries])
         free = self.cache.free_pages()
         if any(n > f for n, f in zip(need, free)):
             raise OutOfPages(f"the step needs {need} pages per group, {free} are free")

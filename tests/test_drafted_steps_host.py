@@ -159,3 +159,34 @@ def test_pages_of_accepted_nodes_stay(monkeypatch):
     run.step_tree([chain(0, 30)], [row()])
     assert run.cache.get(0).num_tokens == 50 and len(run.cache.get(0).tables[0]) == 4
     run.cache.check()
+
+
+def test_forks_that_write_in_one_step_need_a_copy_less(monkeypatch):
+    """Of all owners of a page the last that writes keeps it: a step of all of them needs one copy less than it has owners."""
+    steps.host(monkeypatch)
+    for step in ("tokens", "trees"):
+        run = steps.runner(max_tokens=64)                         # four pages
+        run.storage.copy_pages = lambda: run.cache.take_copies()
+        steps.put(run, "a", 20)
+        for new in ("b", "c"):
+            run.cache.fork("a", new)
+        assert run.cache.free_pages() == [2]                      # copies for two of the three
+        if step == "trees":
+            run.step_tree([chain(r, 2) for r in "abc"], [row() for _ in "abc"])
+        else:
+            run._prepare([StepEntry(r, [1], [0]) for r in "abc"])
+        run.cache.check()
+        assert run.cache.free_pages() == [0] and len({run.cache.get(r).tables[0][1] for r in "abc"}) == 3
+        # an owner that does not write keeps the page: every writer needs a copy
+        run = steps.runner(max_tokens=48)
+        run.storage.copy_pages = lambda: run.cache.take_copies()
+        steps.put(run, "a", 20)
+        for new in ("b", "c"):
+            run.cache.fork("a", new)
+        with pytest.raises(OutOfPages):
+            if step == "trees":
+                run.step_tree([chain(r, 2) for r in "bc"], [row() for _ in "bc"])
+            else:
+                run._prepare([StepEntry(r, [1], [0]) for r in "bc"])
+        assert run.cache.free_pages() == [1] and not run.cache.has_copies
+        run.cache.check()
