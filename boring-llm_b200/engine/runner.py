@@ -160,6 +160,13 @@ class _StepGraph:
         self.kernels = ops.launch_count - before
 
 
+def tree_shape(T: int, R: int, per_request: int):
+    """The (nodes, requests) that a captured step of drafted trees is padded to: it follows from the numbers alone, however many of the nodes
+    are padding, so steps of the same requests share a few shapes. Padding nodes stand in requests of `per_request` behind the others."""
+    step = 16 if T <= 64 else 64
+    return -(-T // step) * step, -(-R // 8) * 8 - (-(step - 1) // per_request)
+
+
 class _TreeBatch:
     """The buffers of a step of drafted trees for T nodes of R requests, and the step itself: forward pass, a token sampled behind every
     node, acceptance and the moves of the accepted rows in the caches of all groups. May be captured and replayed."""
@@ -224,17 +231,21 @@ class _TreeBatch:
                 h["uniform"][at] = np.asarray(numbers, dtype=np.float32)[depth]
             draws.append(states)
             t0 += n
-        R, pads = len(entries), self.T - n_all
-        h["mask"][t0:] = 1
-        for name in ("token_ids", "positions", "cache_rows", "top_k"):
+        # Padding nodes: requests without committed tokens, each node sees itself alone. Their rows lie on the spare page, as often as their
+        # table needs it (rows that coincide get the same numbers). Then requests without nodes.
+        R, pads, each = len(entries), self.T - n_all, runner.tree_padding
+        nth = np.arange(pads, dtype=np.int32)
+        at = nth % each
+        h["mask"][t0:] = np.left_shift(np.uint64(1), at.astype(np.uint64))
+        for name in ("token_ids", "positions", "top_k"):
             h[name][t0:] = 0
+        h["cache_rows"][t0:] = at
         h["temperature"][t0:] = 0.0
-        h["tok_req"][t0:] = np.arange(R, R + pads, dtype=np.int32)
-        h["cu_q"][R:R + pads + 1] = np.arange(t0, self.T + 1, dtype=np.int32)
-        h["cu_q"][R + pads + 1:] = self.T
-        h["ctx_len"][R:] = 1
+        h["tok_req"][t0:] = R + nth // each
+        h["cu_q"][R:] = np.minimum(t0 + each * np.arange(self.R + 1 - R, dtype=np.int32), self.T)
+        h["ctx_len"][R:] = np.diff(h["cu_q"][R:])
         h["slots"][R:] = runner.storage.trash_slot
-        h["tables"][:, R:, 0] = runner.storage.trash_page
+        h["tables"][:, R:, :-(-each // runner.options.page_size)] = runner.storage.trash_page
         return draws
 
     def run(self, runner: "ModelRunner") -> None:
@@ -820,6 +831,11 @@ class ModelRunner:
             self._takes_trees = bool(getattr(self.model, "takes_trees", False))
         return self._takes_trees
 
+    @property
+    def tree_padding(self) -> int:
+        """Padding nodes of one request of a step of drafted trees: what a mask has bits for, and a table has room for."""
+        return min(MAX_NODES, self._table_width * self.options.page_size)
+
     def step_tree(self, entries: Sequence[TreeEntry], rows) -> List[List[int]]:
         """Runs a tree of drafted tokens for each entry's request, samples a token behind every node, and keeps of each tree the longest path
         from node 0 whose tokens are the sampled ones. Returns, per entry, the tokens sampled along that path (one more than
@@ -866,9 +882,7 @@ class ModelRunner:
         shape = None
         try:
             if self._graphs_usable(entries) and T <= TREE_GRAPH_MAX_NODES:
-                # padded to a shape that other steps share: each padding node a request of its own on the spare page, then empty requests
-                T_b = -(-T // 16) * 16 if T <= 64 else -(-T // 64) * 64
-                shape = (T_b, -(-(R + T_b - T) // 8) * 8)
+                shape = tree_shape(T, R, self.tree_padding)
                 batch = self._tree_graphs.pop(shape, None)
                 if batch is None and len(self._tree_graphs) >= STEP_GRAPH_CACHE:
                     del self._tree_graphs[next(iter(self._tree_graphs))]

@@ -190,3 +190,66 @@ def test_forks_that_write_in_one_step_need_a_copy_less(monkeypatch):
                 run._prepare([StepEntry(r, [1], [0]) for r in "bc"])
         assert run.cache.free_pages() == [1] and not run.cache.has_copies
         run.cache.check()
+
+
+# ---- padded steps ----------------------------------------------------------------------------------------------------------
+
+
+def test_padded_tree_steps_share_their_shapes(monkeypatch):
+    """Eight requests with up to 31 drafted tokens each, step by step: a shape for each padded number of nodes, captured once each."""
+    import random
+    rng = random.Random(0)
+    steps.host(monkeypatch)
+    run = steps.runner(max_num_seqs=64, max_tokens=64 * 256)
+    for i in range(32):
+        steps.put(run, i, 20)
+    for _ in range(300):
+        run.step_tree([chain(i, rng.randint(1, 32)) for i in range(8)], [row()] * 8)
+        for i in range(8):
+            run.truncate(i, 20)
+    assert len(set(steps.Batch.made)) == len(steps.Batch.made) <= 7
+    assert len(set(steps.Batch.captured)) == len(steps.Batch.captured) <= 7
+    steps.Batch.made.clear()
+    for requests in list(range(1, 33)) * 4:
+        run.step_tree([chain(i, rng.randint(1, 512 // requests if requests > 8 else 32)) for i in range(requests)], [row()] * requests)
+        for i in range(requests):
+            run.truncate(i, 20)
+    assert len(steps.Batch.made) == len(set(steps.Batch.made)) <= 40                  # none was thrown out and made again
+
+
+@pytest.mark.parametrize("ctx_size,page", [(256, 16), (24, 1), (40, 5), (64, 64)])
+@pytest.mark.parametrize("counts", [[1], [8], [3, 5, 1], [16], [13] * 5, [1] * 16, [20, 20, 20, 7]])
+def test_the_padding_of_a_tree_step_is_a_step_of_its_own(monkeypatch, counts, ctx_size, page):
+    """Padding nodes stand in requests of at most 64 on the spare page: each sees itself, in a row that it writes, that its table holds and that
+    lies inside its request's length; no request of the step is touched by them."""
+    checked = []
+
+    def says(batch, R):
+        h, T, live = batch.h, batch.T, sum(counts)
+        begin, ends = h["cu_q"][:-1], h["cu_q"][1:]
+        n = ends - begin
+        assert h["cu_q"][0] == 0 and ends[-1] == T and (n >= 0).all() and (n <= 64).all()
+        assert list(n[:R]) == counts and ends[R - 1] == live
+        for t in range(live, T):
+            r = int(h["tok_req"][t])
+            assert r >= R and begin[r] <= t < ends[r]
+            node, c = t - begin[r], h["ctx_len"][r] - n[r]
+            assert int(h["mask"][t]) == 1 << int(node) and c == 0
+            at = int(h["cache_rows"][t])
+            assert at == c + node and h["positions"][t] == 0 and h["slots"][r] == run.storage.trash_slot
+            assert at // page < h["tables"].shape[2] and (h["tables"][:, r, at // page] == run.storage.trash_page).all()
+        for r in range(R, len(n)):
+            assert h["ctx_len"][r] >= n[r]
+        checked.append(T)
+        return steps.only_node_0(batch, R)
+    steps.host(monkeypatch, says)
+    if max(counts) > ctx_size // 2:
+        pytest.skip("more nodes than the context holds")
+    run = steps.runner(ctx_size=ctx_size, page_size=page)
+    for i in range(len(counts)):
+        steps.put(run, i, 3)
+    for _ in range(3):
+        run.step_tree([chain(i, n) for i, n in enumerate(counts)], [row()] * len(counts))
+        for i in range(len(counts)):
+            run.truncate(i, 3)
+    assert len(checked) == 3 and checked[0] % 16 == 0 and checked[0] - sum(counts) < 64
