@@ -47,7 +47,6 @@ class Engine:
             raise ValueError("draft_tokens: this model's mixers keep state of their own beside pages, or attend in a way of their own; "
                              "drafted tokens could not be taken back")
         self._ids = itertools.count()
-        self._early: List[Request] = []       # finished when a fork read the step ahead: the next step returns them
         self._inflight = None                 # (scheduled step, PendingDecode): launched, tokens not read yet
         self.stats_time = {"engine_steps": 0, "step_seconds": 0.0}
 
@@ -85,7 +84,7 @@ class Engine:
         has then already got a row in the step after; that row's result is dropped (the reference's loop,
         src/model.br:2293-2304, feeds no token after the end token either: nothing of the row is kept)."""
         done = self._step()
-        early, self._early = self._early, []
+        early, self.scheduler.unreported = self.scheduler.unreported, []
         return early + done
 
     def _step(self) -> List[Request]:
@@ -148,7 +147,7 @@ class Engine:
     def fork(self, request, params: Optional[SamplingParams] = None, request_id=None) -> Request:
         """A second running request that goes on from where `request` (a `Request` that runs, its prompt computed) is, with parameters
         and a generator of its own. The pages of what both have in common are shared."""
-        self._early += self.drain()
+        self.scheduler.unreported += self.drain()
         if request.state != RUNNING or request.remaining != 1:
             raise ValueError(f"request {request.request_id!r} cannot be forked: it has ended, or its prompt is not computed yet")
         return self._fork(request, params if params is not None else copy.copy(request.params), request_id, request.num_computed,
@@ -195,9 +194,9 @@ class Engine:
 
     def run_until_done(self) -> None:
         while self.scheduler.has_work():
-            before = (len(self.scheduler.waiting), len(self.scheduler.running), len(self.scheduler.finished))
+            before = self.scheduler.progress()
             self.step()
-            after = (len(self.scheduler.waiting), len(self.scheduler.running), len(self.scheduler.finished))
+            after = self.scheduler.progress()
             if before == after and not self.scheduler.running:
                 raise RuntimeError("the scheduler made no progress with requests still waiting")
 

@@ -87,6 +87,7 @@ class Scheduler:
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []          # in admission order: oldest first
         self.finished: Dict[object, Request] = {}
+        self.unreported: List[Request] = []       # ended when a fork read the step ahead: the engine's next step returns them
         self._arrivals = itertools.count()
         self.num_preemptions = 0
 
@@ -128,7 +129,12 @@ class Scheduler:
                 return
 
     def has_work(self) -> bool:
-        return bool(self.waiting or self.running)
+        """Whether there is something for a step to do, or to return."""
+        return bool(self.waiting or self.running or self.unreported)
+
+    def progress(self) -> tuple:
+        """Changes with every step that admits, ends or returns a request."""
+        return len(self.waiting), len(self.running), len(self.finished), len(self.unreported)
 
     # ---- one step ----------------------------------------------------------------------------------
     def schedule(self) -> Optional[ScheduledStep]:

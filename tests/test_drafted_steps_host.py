@@ -253,3 +253,30 @@ def test_the_padding_of_a_tree_step_is_a_step_of_its_own(monkeypatch, counts, ct
         for i in range(len(counts)):
             run.truncate(i, 3)
     assert len(checked) == 3 and checked[0] % 16 == 0 and checked[0] - sum(counts) < 64
+
+
+# ---- requests and options ------------------------------------------------------------------------------------------------
+
+
+def test_what_ended_in_front_of_a_refused_fork_is_still_handed_out(monkeypatch):
+    """A request that ends in the step that a fork reads first is work until a step has returned it, also when the fork is refused."""
+    steps.host(monkeypatch)
+    eng = steps.engine(monkeypatch, draft_tokens=0)
+    req = steps.hold(eng, [1, 2, 3, 4], SamplingParams(n_predict=2, ignore_eos=True))
+    sched = eng.scheduler.schedule()
+    eng.runner.cache.commit(req.request_id, 1)
+    eng._inflight = (sched, None)
+    eng.runner.collect_decode = lambda pending: [5]
+    with pytest.raises(ValueError):
+        eng.fork(req)
+    assert req.state == FINISHED and eng.scheduler.has_work()
+    assert eng.step() == [req] and not eng.scheduler.has_work() and eng.step() == []
+    # `run_until_done` takes it as well
+    req = steps.hold(eng, [1, 2, 3, 4], SamplingParams(n_predict=2, ignore_eos=True))
+    sched = eng.scheduler.schedule()
+    eng.runner.cache.commit(req.request_id, 1)
+    eng._inflight = (sched, None)
+    with pytest.raises(ValueError):
+        eng.fork(req)
+    eng.run_until_done()
+    assert not eng.scheduler.has_work()
