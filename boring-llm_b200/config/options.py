@@ -22,9 +22,10 @@ class EngineOptions:
     cuda_graphs: bool = True            # replay captured decode steps
     step_graph_after: int = 2           # capture a general step's padded shape when it comes this many times (0: never)
     lookahead: bool = True              # launch the next decode step (its tokens taken on the device) before this one's are read
-    draft_tokens: int = 0               # most tokens that are drafted for a request and step, from its own text (0: none; at most 63)
     debug_poison: bool = False          # fill pages with NaN when they are given back: a read past a request's length shows
     device: str = "cuda:0"
+    # most tokens that are drafted for a request and step, from its own text (0: none; at most 63)
+    draft_tokens: int = 0
 
     def __post_init__(self):
         if self.dtype in ("bf16",):

@@ -280,3 +280,8 @@ def test_what_ended_in_front_of_a_refused_fork_is_still_handed_out(monkeypatch):
         eng.fork(req)
     eng.run_until_done()
     assert not eng.scheduler.has_work()
+
+
+def test_positional_options_stand_where_they_stood():
+    o = EngineOptions("bfloat16", 16, 0, 4096, 64, 2048, 512, True, 2, True, True, "cuda:1")
+    assert o.debug_poison is True and o.device == "cuda:1" and o.draft_tokens == 0
