@@ -331,6 +331,7 @@ class Scheduler:
     def _finish(self, req: Request, reason: str, live: bool) -> None:
         req.state = FINISHED
         req.finish_reason = reason
+        req.history = None                        # some 600 bytes a token, and a finished request is kept
         if live and req.request_id in self.cache:
             self.cache.free(req.request_id)
         self.finished[req.request_id] = req

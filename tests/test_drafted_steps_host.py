@@ -285,3 +285,14 @@ def test_what_ended_in_front_of_a_refused_fork_is_still_handed_out(monkeypatch):
 def test_positional_options_stand_where_they_stood():
     o = EngineOptions("bfloat16", 16, 0, 4096, 64, 2048, 512, True, 2, True, True, "cuda:1")
     assert o.debug_poison is True and o.device == "cuda:1" and o.draft_tokens == 0
+
+
+def test_a_finished_request_keeps_no_drafting_index(monkeypatch):
+    steps.host(monkeypatch, steps.whole_chains)
+    eng = steps.engine(monkeypatch)
+    req = steps.hold(eng, [1, 2, 3, 1, 2, 3], SamplingParams(n_predict=3, ignore_eos=True))
+    assert eng.step() == [req] and req.output == [1, 7, 7] and req.history is None
+    req = steps.hold(eng, [1, 2, 3, 1, 2, 3], SamplingParams(n_predict=30, ignore_eos=True))
+    assert eng.step() == [] and req.history is not None
+    eng.scheduler.abort(req.request_id)
+    assert req.history is None and eng.scheduler.finished[req.request_id] is req
