@@ -2340,10 +2340,10 @@ def copy_blocks(tensors, pairs) -> None:
     blocks are contiguous: pages, or state slots, of all layers in one launch (a launch for every 1,024 pairs). No block may be the
     target of two copies, or target and source. The pairs are part of the launch: a captured call copies the same ones again."""
     try:
-        flat = array.array("i", itertools.chain.from_iterable(pairs))
+        flat, longest = array.array("i", itertools.chain.from_iterable(pairs)), max(map(len, pairs), default=2)
     except (OverflowError, TypeError) as e:
         raise KernelError(f"pairs: must be pairs of block numbers ({e})") from None
-    if len(flat) != 2 * len(pairs):
+    if len(flat) != 2 * len(pairs) or longest != 2:
         raise KernelError("pairs: must be pairs of block numbers")
     lists = array.array("q")
     for i, t in enumerate(tensors):

@@ -296,3 +296,10 @@ def test_a_finished_request_keeps_no_drafting_index(monkeypatch):
     assert eng.step() == [] and req.history is not None
     eng.scheduler.abort(req.request_id)
     assert req.history is None and eng.scheduler.finished[req.request_id] is req
+
+
+@pytest.mark.parametrize("pairs", [[(1, 2, 3), (4,)], [(0, 1), (2, 3, 4), (5,)], [(), (0, 1, 2, 3)]])
+def test_copies_that_are_no_pairs_are_refused(pairs):
+    """As many numbers as pairs have, but not two by two."""
+    with pytest.raises(KernelError, match="pairs"):
+        ops.copy_blocks([torch.zeros(2, 9, 4)], pairs)
