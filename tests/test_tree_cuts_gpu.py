@@ -118,3 +118,77 @@ def test_steps_of_many_nodes(model_folders, cuda_graphs):
         generation.check_greedy(d, prompts[i], said[i], "bfloat16")
     run.check_kernels()
     assert (run.graph_steps > 0) == cuda_graphs
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,dh", [(28, 4, 128), (14, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("counts,committed", [([64], [6000]), ([64, 33, 40], [3000, 1500, 2501]), ([64, 50, 20, 64, 37, 36, 5, 64], [700 + 61 * r for r in range(8)])])
+def test_units_of_two_tiles_that_are_cut(counts, committed, H, KV, dh, dtype):
+    """64 nodes of 7 or 8 query heads are a unit of two row tiles (of 126 or 128 rows) and what is left of the nodes: over few requests every unit lies in
+    several blocks, whose parts of both tiles are merged; few parts and many."""
+    check(TreeStep(counts, committed, H, KV, dh, 16, dtype, 31, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window", [460, 1000, 2049])
+@pytest.mark.parametrize("H,KV,dh,counts,committed", [(4, 2, 64, [13, 30, 1], [3000, 1500, 2501]), (28, 4, 128, [64, 40], [2500, 2300]), (16, 2, 128, [24, 17, 64], [4003, 999, 30])])
+def test_windows_that_are_cut(H, KV, dh, counts, committed, window, dtype):
+    """Windows of more key blocks than a unit has that is never cut; the pages that they have passed hold NaN."""
+    s = TreeStep(counts, committed, H, KV, dh, 16, dtype, 32, device=DEV)
+    for r, c in enumerate(committed):
+        for i in range(max(0, c - window + 1) // 16):
+            s.k[s.table[r, i].long()] = float("nan")
+            s.v[s.table[r, i].long()] = float("nan")
+    check(s, window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,dh", [(28, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("window", [0, 130])
+def test_units_of_one_and_two_tiles_in_turn(H, KV, dh, window, dtype):
+    """More units than blocks, of one and of two tiles, of one key block and of several: a block goes through all of them in one pipeline."""
+    rng = np.random.default_rng(5)
+    counts = [int(n) for n in rng.choice([1, 5, 17, 18, 19, 35, 36, 37, 40, 54, 55, 64], 120)]
+    committed = [int(c) for c in rng.choice([0, 1, 15, 50, 63, 64, 130, 200, 330, 420], 120)]
+    check(TreeStep(counts, committed, H, KV, dh, 16, dtype, 33, device=DEV), window)
+
+
+@pytest.mark.parametrize("rows", [256, 333, 700])
+@pytest.mark.parametrize("H,KV,dh,d", [(14, 2, 64, 896), (16, 2, 128, 264), (4, 2, 64, 128)])
+def test_the_product_on_pairs_writes_rows_beside_positions(rows, H, KV, dh, d):
+    """Keys and values lie in the cache rows that it is given, rotated by the step's table, whose positions are others; nothing else is written.
+    Against the formula in 64 bits: a sum of d products and a bias in 32 bits, (d + 1) 2^-24 of the sum of magnitudes, two products and a sum of
+    the rotation (3 x 2^-24 more), then one rounding to bfloat16."""
+    o = ops()
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    width, page, requests = (H + 2 * KV) * dh, 16, 5
+    tok_req = torch.sort(torch.randint(0, requests, (rows,), generator=g, device=DEV)).values.to(torch.int32)
+    per = -(-rows // page) + 2
+    table = torch.randperm(requests * per, generator=g, device=DEV).to(torch.int32).view(requests, per)
+    positions = torch.randint(0, 900, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    cache_rows = torch.cat([torch.randperm(n, generator=g, device=DEV) + 7 for n in torch.bincount(tok_req, minlength=requests).tolist()]).to(torch.int32)
+    inv = 10000.0 ** (-torch.arange(dh // 2, device=DEV).float() / (dh // 2))
+    x = (torch.randn(rows, d, generator=g, device=DEV) * 0.5).bfloat16()
+    w = (torch.randn(width, d, generator=g, device=DEV) / d ** 0.5).bfloat16()
+    b = torch.randn(width, generator=g, device=DEV).bfloat16()
+    assert o.qkv_rope_tc_supported(x, w, H, KV, dh, page)
+    cs, sn = o.rope_table(positions, inv, dh // 2, 1.0)
+    q = torch.empty(rows, H * dh, dtype=torch.bfloat16, device=DEV)
+    k = torch.full((requests * per, KV, page, dh), float("nan"), dtype=torch.bfloat16, device=DEV)
+    v = k.clone()
+    o.qkv_rope_tc(x, w, b, cache_rows, tok_req, table, cs, sn, q, k, v, H, KV, dh)
+    full = x.double() @ w.double().T + b.double()
+    mags = (x.double().abs() @ w.double().abs().T + b.double().abs()) * (d + 4) * 2.0 ** -24
+    full, mags = full.view(rows, H + 2 * KV, dh), mags.view(rows, H + 2 * KV, dh)
+    c, s = cs.double()[:, None], sn.double()[:, None]
+    lo, hi = full[..., :dh // 2], full[..., dh // 2:]
+    turned = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+    slack = torch.cat([mags[..., :dh // 2] * c.abs() + mags[..., dh // 2:] * s.abs(), mags[..., dh // 2:] * c.abs() + mags[..., :dh // 2] * s.abs()], -1)
+    at = table[tok_req.long(), (cache_rows // page).long()].long(), (cache_rows % page).long()
+    for got, want, room in ((q.view(rows, H, dh), turned[:, :H], slack[:, :H]), (k[at[0], :, at[1]], turned[:, H:H + KV], slack[:, H:H + KV]),
+                            (v[at[0], :, at[1]], full[:, H + KV:], mags[:, H + KV:])):
+        assert ((got.double() - want).abs() <= room * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()).all()
+    written = torch.zeros(requests * per, page, dtype=torch.bool, device=DEV)
+    written[at] = True
+    for t in (k, v):
+        assert torch.isnan(t.transpose(1, 2)[~written]).all()
