@@ -842,7 +842,10 @@ class ModelRunner:
         there were drafted tokens on it): the same that one step after the other would have sampled, from the same random numbers.
         All but the last are in the cache then, behind the token of node 0. `rows` holds one (params, generator, history)
         per entry; a repeat penalty is refused (StepError), as is a model that keeps more of a request than pages. A step that fails, also
-        when a kernel has given up on a bounded wait (looked at here, before anything is kept), leaves requests and generators as they were."""
+        when a kernel has given up on a bounded wait (looked at here, before anything is kept), leaves requests and generators as they were.
+        A step takes nodes x vocabulary x 4 bytes for its logits (the scheduler's drafts stay within TREE_GRAPH_MAX_NODES nodes: 311 MB at a
+        vocabulary of 151,936); more nodes than that, and steps in 32 bits, are launched kernel by kernel. In 32 bits the tokens are the same ones
+        exactly; in bfloat16 a step of many nodes runs other kernels than a step of one token, and a near tie may fall the other way."""
         if not self.takes_trees:
             raise StepError("this model does not run trees of drafted tokens: a mixer keeps state, or attends in a way of its own")
         if not entries or len(rows) != len(entries):

@@ -30,7 +30,7 @@ from ..cache import CacheManager
 from ..config import EngineOptions
 from ..sampling.params import SamplingParams, XorShift64
 from .draft import History
-from .runner import StepEntry
+from .runner import TREE_GRAPH_MAX_NODES, StepEntry
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
 
@@ -234,12 +234,13 @@ class Scheduler:
     def draft(self, step: ScheduledStep) -> Optional[List[tuple]]:
         """(tokens, parents) of a tree of drafted tokens for every request of a step that only decodes, or None: it is another kind
         of step, a request has a penalty on repeated tokens (its tokens would have to be sampled one after the other), or
-        nothing is drafted for any. The trees respect the token budget, the context and what each request may still say."""
+        nothing is drafted for any. The trees respect the token budget, the context and what each request may still say, and have
+        no more nodes together than a captured step takes: there is a row of logits for every one of them."""
         if not step.entries or not all(s and len(e.tokens) == 1 for e, s in zip(step.entries, step.samples)):
             return None
         if any(r.params.repeat_penalty != 1.0 for r in step.requests):
             return None
-        room = self.options.max_num_batched_tokens // len(step.requests)
+        room = min(self.options.max_num_batched_tokens, TREE_GRAPH_MAX_NODES) // len(step.requests)
         trees, drafted = [], 0
         for req in step.requests:
             if req.history is None:

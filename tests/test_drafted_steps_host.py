@@ -303,3 +303,23 @@ def test_copies_that_are_no_pairs_are_refused(pairs):
     """As many numbers as pairs have, but not two by two."""
     with pytest.raises(KernelError, match="pairs"):
         ops.copy_blocks([torch.zeros(2, 9, 4)], pairs)
+
+
+@pytest.mark.parametrize("requests,budget,each", [(1, 2048, 64), (8, 2048, 64), (9, 2048, 56), (64, 2048, 8), (64, 256, 4), (600, 2048, None)])
+def test_drafts_of_a_step_stay_within_a_captured_one(requests, budget, each):
+    """Every node has a row of logits: however many requests draft, a step has no more nodes than a captured one takes."""
+    o = EngineOptions(ctx_size=256, max_num_seqs=requests, max_tokens=requests * 32, max_num_batched_tokens=max(budget, 6 * requests), prefill_chunk=6, draft_tokens=63)
+    s = Scheduler(CacheManager([FULL], 16, o.capacity_tokens, requests), o)
+    for i in range(requests):
+        s.add(i, [1, 2, 3, 1, 2, 3], SamplingParams(n_predict=100))
+    while s.waiting:
+        step = s.schedule()
+        for e in step.entries:
+            s.cache.commit(e.request_id, len(e.tokens))
+        s.apply(step, [1 if len(e.tokens) > 1 else 2 for e, said in zip(step.entries, step.samples) if said])
+    s.options.max_num_batched_tokens = max(budget, requests)
+    trees = s.draft(s.schedule())
+    if each is None:
+        assert trees is None
+    else:
+        assert [len(t) for t, _ in trees] == [each] * requests and requests * each <= 512
