@@ -24,7 +24,8 @@ class EngineOptions:
     lookahead: bool = True              # launch the next decode step (its tokens taken on the device) before this one's are read
     debug_poison: bool = False          # fill pages with NaN when they are given back: a read past a request's length shows
     device: str = "cuda:0"
-    # most tokens that are drafted for a request and step, from its own text (0: none; at most 63)
+    # most tokens that are drafted for a request and step, from its own text (0: none; at most 63); for few requests whose text repeats
+    # itself. With it no step is launched ahead, also where nothing is drafted, whatever `lookahead` says
     draft_tokens: int = 0
 
     def __post_init__(self):

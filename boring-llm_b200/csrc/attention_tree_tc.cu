@@ -20,10 +20,11 @@
 // P is rounded to bfloat16 (half a step, 2^-8 of each weight, as the operand of a bfloat16 product must be); the sum is of the 32-bit values.
 //
 // What bounds it: with two full tiles the products and the hand-overs between the warps together. 64 requests of 64 nodes, 28 / 4 heads of
-// 128, contexts of 2,003 to 4,001: 217 us, 734 TFLOP/s (840 with the rows that tiles lack); without the softmax's arithmetic 195, without copies 207, without both 167, of which
-// S is 50 (an MMA of N 64 reads 6 KB of shared memory in 32 cycles, more than the 4 KB there are; a key block of 128 would need
-// the tensor memory that the second pair of score buffers has) and P V 15. With one request or few, the chains at the ends: lengths, pages, first
-// copies (5 us), outputs and the merge (4 to 10 us). Tried: key blocks of 128 in two passes over the scores 1.3 times as long; one group of row warps
+// 128, contexts of 2,003 to 4,001: 220 us in a row of captured calls, 724 TFLOP/s (827 with the rows that tiles lack); 260 us and 612 in long runs, where the power
+// cap takes the clock down. The launch by itself 208 us and the merge 20, of which most lies under its end. 16 such requests (profiler, 75 us): the tensor pipes are
+// active in 46 % of the cycles, DRAM at 28 % of its rate. An MMA of N 64 reads 6 KB of shared memory in 32 cycles, more than the 4 KB that there are; a key block of
+// 128 would need the tensor memory that the second pair of score buffers has. With one request or few, the chains at the ends: lengths, pages, first
+// copies and scores (3 us), outputs (1) and the merge (7 to 14 us by itself). Tried: key blocks of 128 in two passes over the scores 1.3 times as long; one group of row warps
 // 1.6 times; 2^x by polynomials on the FMA pipes, scalar arithmetic, other orders of the exponentials: nothing.
 //
 // Every wait on an mbarrier is bounded; a block whose bound runs out records a code in a status word
