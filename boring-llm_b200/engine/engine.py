@@ -82,7 +82,10 @@ class Engine:
         read (`EngineOptions.lookahead`): the device feeds the sampled tokens back itself, the host reads them one
         step behind, and the GPU does not wait for the host between steps. A request that ends with an end token
         has then already got a row in the step after; that row's result is dropped (the reference's loop,
-        src/model.br:2293-2304, feeds no token after the end token either: nothing of the row is kept)."""
+        src/model.br:2293-2304, feeds no token after the end token either: nothing of the row is kept).
+
+        When a step fails, requests whose tokens are in the cache already end with the reason "error"; the others, those of a step of drafted
+        trees among them, are as they were before it."""
         done = self._step()
         early, self.scheduler.unreported = self.scheduler.unreported, []
         return early + done
